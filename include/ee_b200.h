@@ -451,6 +451,75 @@ EE_API int ee_kv_decode_attention(const ee_kv_cache* cache, const void* q, int64
                                   const void* k_new, const void* v_new, int64_t ld_new, float scale, void* out,
                                   int64_t ldo, float* H, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Paged KV cache: sequences of different lengths in pages of page_size tokens (16, 32, 64 or
+ * 128), for prefill in chunks, decode steps of many sequences and everything between.
+ *   tier EE_INT8 / EE_FP8: block j of a sequence (tokens j P .. j P + P - 1) is kept as 8-bit
+ *     codes in page table[seq][j], with one fp32 scale per KV head for its keys and one for
+ *     its values, s = max |x| / 127 (or / 448), code = rn(x / s), once all its tokens are
+ *     there.  Until then its tokens are kept in fp16 in the sequence's open buffer, and the
+ *     block before it keeps its fp16 rows too: up to page_size tokens can be taken back
+ *     exactly.  What the cache holds depends on the tokens, not on how they were appended.
+ *   tier EE_FP16: fp16 in the pages.
+ * A value that is not finite makes its block's scale infinite and the rows that see the
+ * block NaN.  The order of the values inside a page is the kernels' own; ee_paged_read gives
+ * the rows back.  Memory: ee_paged_cache_bytes (0 for a shape outside the limits), laid out
+ * by ee_paged_cache_init, which empties the table (-1).  The caller hands pages out by
+ * writing page numbers into `table`; a page belongs to one sequence that is written to. */
+typedef struct ee_paged_cache {
+  int64_t num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages;
+  int32_t tier;
+  uint8_t* pages; /* [num_pages, kv_heads, 2 (K, V), page_size * head_dim] codes or fp16 */
+  float* scale;   /* [num_pages, kv_heads, 2 (K, V)]; 8-bit tiers */
+  void* open;     /* fp16 [max_seqs, 2, kv_heads, 2 (K, V), page_size * head_dim]; 8-bit tiers */
+  int32_t* table; /* [max_seqs, max_pages] page of each block, -1: none */
+} ee_paged_cache;
+
+/* The sequences of one call, as device arrays: entry b is sequence seq[b] (each at most once
+ * in an append), whose rows cu[b] .. cu[b + 1] - 1 are its tokens at positions start[b] ..;
+ * length[b] is the sequence's length with those tokens (for ee_paged_append and
+ * ee_paged_attention start + count).  rows = cu[batch]; max_new, the largest count, only
+ * chooses the kernel.  An entry outside the cache is left alone, and a token whose block has
+ * no page is not stored (a hole, which attention skips and ee_paged_read gives as zeros);
+ * both set the device error word (ee_device_check, bit 16). */
+typedef struct ee_paged_step {
+  int64_t batch, rows, max_new;
+  const int32_t* seq;
+  const int32_t* start;
+  const int32_t* length;
+  const int32_t* cu;
+} ee_paged_step;
+
+EE_API size_t ee_paged_cache_bytes(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size,
+                                   int64_t max_seqs, int64_t max_pages, int tier);
+EE_API int ee_paged_cache_init(ee_paged_cache* cache, void* memory, size_t bytes, int64_t num_pages, int64_t kv_heads,
+                               int64_t head_dim, int64_t page_size, int64_t max_seqs, int64_t max_pages, int tier,
+                               void* stream);
+/* Appends the step's rows: k, v fp16 [rows, kv_heads * head_dim] (row strides ldk / ldv).
+ * With cos / sin (fp16 [rows, head_dim], row stride ld_cs; both or neither) k is rotated on
+ * the way, y_j = x_j cos_j + rot_j sin_j with rot = (-x[d/2 ..], x[.. d/2]) in fp32, rounded
+ * to fp16 once, and so is q (fp16 [rows, heads * head_dim], nullable) into q_out, which may be
+ * q itself.  Without them q is copied. */
+EE_API int ee_paged_append(const ee_paged_cache* cache, const ee_paged_step* step, const void* k, int64_t ldk,
+                           const void* v, int64_t ldv, const void* cos, const void* sin, int64_t ld_cs, const void* q,
+                           int64_t ldq, int64_t heads, void* q_out, int64_t ldqo, void* stream);
+/* Rows of the span back as fp16 (code * s, rounded once): k, v [rows, kv_heads * head_dim].
+ * length[b] is the sequence's current length: it says which blocks are still open. */
+EE_API int ee_paged_read(const ee_paged_cache* cache, const ee_paged_step* step, void* k, int64_t ldk, void* v,
+                         int64_t ldv, void* stream);
+/* Causal attention of the step's query rows (fp16 q [rows, heads * head_dim], rotated; heads a
+ * multiple of kv_heads) after their append: the row at position p sees keys 0 .. p.  out fp16
+ * [rows, heads * head_dim] = softmax(scale q k) v, H (nullable, fp32 [rows, heads]) the entropy
+ * of each softmax row in nats; a row that sees no key gives zeros.  One launch, whatever the
+ * lengths: the keys are dealt to the CTAs in even shares, and a unit's last CTA joins its
+ * parts in a fixed order (the same bits every time).  workspace: ee_paged_workspace_bytes, its
+ * first ee_paged_workspace_head_bytes() zeroed once (every call leaves them zero); one
+ * workspace serves one call at a time. */
+EE_API size_t ee_paged_workspace_bytes(const ee_paged_cache* cache);
+EE_API size_t ee_paged_workspace_head_bytes(void);
+EE_API int ee_paged_attention(const ee_paged_cache* cache, const ee_paged_step* step, const void* q, int64_t ldq,
+                              int64_t heads, float scale, void* out, int64_t ldo, float* H, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- decoder-stack engine
  * The whole decoder stack of a Llama-architecture model for one fixed batch shape
  * [batch, seq] as one native object: the reference's Python layer loop

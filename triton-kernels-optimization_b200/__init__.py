@@ -10,8 +10,9 @@ hand-written tcgen05 / TMA kernels behind the C ABI of
 so it is imported through ``__graft_entry__.load_package()`` (module name
 ``tko_b200``).
 """
-from . import _lib, kvcache, packfile, sharding
+from . import _lib, kvcache, packfile, paged, sharding
 from .kvcache import EntropyKVCache
+from .paged import PagedKVCache, PagedStep
 from .dispatch import (
     EntropyDispatchedLinear,
     EntropyRouter,

@@ -463,7 +463,10 @@ const char* ee_last_error(void) { return g_last_error.c_str(); }
 
 int ee_device_check(int* value) {
   int v = 0;
-  if (ee::read_and_clear_device_error(&v) != 0) return fail(EE_ERR_CUDA, "reading the device error word failed");
+  int paged = 0;
+  if (ee::read_and_clear_device_error(&v) != 0 || ee::read_and_clear_paged_error(&paged) != 0)
+    return fail(EE_ERR_CUDA, "reading the device error word failed");
+  v |= paged;
   if (value) *value = v;
   if (v != 0) return fail(EE_ERR_DEVICE, "device error word 0x%x (a bounded wait in a kernel gave up)", v);
   return EE_OK;
@@ -826,6 +829,188 @@ int ee_kv_decode_attention(const ee_kv_cache* cache, const void* q, int64_t ldq,
                                                      kv_splits(cache->batch, cache->kv_heads, cache->max_tokens),
                                                      static_cast<float*>(workspace), out, ldo, H, as_stream(stream)),
                       "kv_decode_attention");
+}
+
+// ------------------------------------------------------------------ paged KV cache
+}  // extern "C"
+namespace {
+struct PagedLayout {
+  size_t pages, scale, open, table, total;
+};
+PagedLayout paged_layout(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t max_seqs,
+                         int64_t max_pages, int tier) {
+  PagedLayout L{};
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += align256(bytes);
+    return at;
+  };
+  const bool wide = tier == EE_FP16;
+  const size_t block = size_t(2) * kv_heads * page_size * head_dim;  // K and V values of a page
+  L.pages = take(size_t(num_pages) * block * (wide ? 2 : 1));
+  L.scale = take(wide ? 0 : size_t(num_pages) * kv_heads * 8);
+  L.open = take(wide ? 0 : size_t(max_seqs) * 2 * block * 2);
+  L.table = take(size_t(max_seqs) * max_pages * 4);
+  L.total = off;
+  return L;
+}
+bool paged_shape_ok(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t max_seqs,
+                    int64_t max_pages, int tier) {
+  return num_pages > 0 && num_pages < (int64_t(1) << 31) && kv_heads > 0 && kv_heads <= 1024 &&
+         (head_dim == 64 || head_dim == 128) &&
+         (page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && max_seqs > 0 &&
+         max_seqs < (int64_t(1) << 24) && max_pages > 0 && max_pages * page_size < (int64_t(1) << 31) &&
+         max_pages * max_seqs < (int64_t(1) << 40) && (tier == EE_INT8 || tier == EE_FP8 || tier == EE_FP16);
+}
+int paged_cache_ok(const ee_paged_cache* c) {
+  if (c == nullptr || c->table == nullptr || c->pages == nullptr ||
+      !paged_shape_ok(c->num_pages, c->kv_heads, c->head_dim, c->page_size, c->max_seqs, c->max_pages, c->tier))
+    return fail(EE_ERR_INVALID, "the paged cache is not initialised");
+  if (c->tier != EE_FP16 && (c->scale == nullptr || c->open == nullptr))
+    return fail(EE_ERR_INVALID, "an 8-bit paged cache needs its scales and open blocks");
+  if (!al16(c->pages) || !al16(c->scale) || !al16(c->open))
+    return fail(EE_ERR_MISALIGNED, "the paged cache's arrays must be 16-byte aligned");
+  return EE_OK;
+}
+int paged_step_ok(const ee_paged_step* st) {
+  if (st == nullptr || st->batch < 0 || st->rows < 0 || st->max_new < 0) return fail(EE_ERR_INVALID, "bad paged step");
+  if (st->rows > kMaxDim || st->batch > kMaxDim) return fail(EE_ERR_UNSUPPORTED, "a step has at most 2^31 - 1 rows");
+  if (st->batch > 0 && (!st->seq || !st->start || !st->length || !st->cu))
+    return fail(EE_ERR_INVALID, "a step's seq, start, length and cu arrays are required");
+  return EE_OK;
+}
+ee::PagedArgs paged_args(const ee_paged_cache& c) {
+  ee::PagedArgs a;
+  a.num_pages = c.num_pages;
+  a.kv_heads = c.kv_heads;
+  a.head_dim = c.head_dim;
+  a.page_size = c.page_size;
+  a.max_seqs = c.max_seqs;
+  a.max_pages = c.max_pages;
+  a.tier = c.tier;
+  a.page_shift = c.page_size == 16 ? 4 : (c.page_size == 32 ? 5 : (c.page_size == 64 ? 6 : 7));
+  a.pages = c.pages;
+  a.scale = c.scale;
+  a.open = static_cast<__half*>(c.open);
+  a.table = c.table;
+  return a;
+}
+ee::PagedStepArgs paged_step_args(const ee_paged_step& s) { return {s.batch, s.rows, s.seq, s.start, s.length, s.cu}; }
+// rows of `width` fp16 values with stride ld that the kernels read and write 16 bytes at a time
+bool rows_ok(const void* p, int64_t ld, int64_t width) { return al16(p) && ld >= width && ld % 8 == 0; }
+// blocks that a step may touch times the KV heads, as CTAs of one launch
+bool paged_grid_ok(const ee_paged_cache& c, const ee_paged_step& st, int64_t more) {
+  return (st.rows / c.page_size + 2 * st.batch) * c.kv_heads + more <= kMaxDim;
+}
+}  // namespace
+extern "C" {
+
+size_t ee_paged_cache_bytes(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t max_seqs,
+                            int64_t max_pages, int tier) {
+  if (!paged_shape_ok(num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages, tier)) return 0;
+  return paged_layout(num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages, tier).total;
+}
+
+int ee_paged_cache_init(ee_paged_cache* cache, void* memory, size_t bytes, int64_t num_pages, int64_t kv_heads,
+                        int64_t head_dim, int64_t page_size, int64_t max_seqs, int64_t max_pages, int tier, void* stream) {
+  if (cache == nullptr) return fail(EE_ERR_INVALID, "cache is NULL");
+  if (!paged_shape_ok(num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages, tier))
+    return fail(EE_ERR_INVALID, "bad paged-cache shape (head_dim 64 / 128, pages of 16 / 32 / 64 / 128 tokens, tier 0 - 2)");
+  const PagedLayout L = paged_layout(num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages, tier);
+  int st = check_ws(memory, bytes, L.total);
+  if (st != EE_OK) return st;
+  uint8_t* p = static_cast<uint8_t*>(memory);
+  cache->num_pages = num_pages;
+  cache->kv_heads = kv_heads;
+  cache->head_dim = head_dim;
+  cache->page_size = page_size;
+  cache->max_seqs = max_seqs;
+  cache->max_pages = max_pages;
+  cache->tier = tier;
+  cache->pages = p + L.pages;
+  cache->scale = tier == EE_FP16 ? nullptr : reinterpret_cast<float*>(p + L.scale);
+  cache->open = tier == EE_FP16 ? nullptr : p + L.open;
+  cache->table = reinterpret_cast<int32_t*>(p + L.table);
+  cudaError_t e = cudaMemsetAsync(cache->table, 0xFF, size_t(max_seqs) * max_pages * 4, as_stream(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "cudaMemsetAsync");
+  return EE_OK;
+}
+
+int ee_paged_append(const ee_paged_cache* cache, const ee_paged_step* step, const void* k, int64_t ldk, const void* v,
+                    int64_t ldv, const void* cos, const void* sin, int64_t ld_cs, const void* q, int64_t ldq,
+                    int64_t heads, void* q_out, int64_t ldqo, void* stream) {
+  int st = paged_cache_ok(cache);
+  if (st == EE_OK) st = paged_step_ok(step);
+  if (st != EE_OK) return st;
+  if (step->batch == 0 || step->rows == 0) return EE_OK;
+  if (!k || !v) return fail(EE_ERR_INVALID, "k and v are required");
+  if ((cos == nullptr) != (sin == nullptr)) return fail(EE_ERR_INVALID, "cos and sin go together");
+  if ((q == nullptr) != (q_out == nullptr)) return fail(EE_ERR_INVALID, "q and q_out go together");
+  const int64_t d = cache->head_dim, row = cache->kv_heads * d;
+  if (!rows_ok(k, ldk, row) || !rows_ok(v, ldv, row))
+    return fail(EE_ERR_MISALIGNED, "K / V rows must be 16-byte aligned with strides >= kv_heads * head_dim, % 8");
+  if (cos && (!rows_ok(cos, ld_cs, d) || !rows_ok(sin, ld_cs, d)))
+    return fail(EE_ERR_MISALIGNED, "cos / sin rows must be 16-byte aligned with a stride >= head_dim, % 8");
+  int64_t vecs = 0;
+  if (q) {
+    if (heads <= 0 || heads > 65536) return fail(EE_ERR_INVALID, "heads must be 1 - 65536");
+    if (!rows_ok(q, ldq, heads * d) || !rows_ok(q_out, ldqo, heads * d))
+      return fail(EE_ERR_MISALIGNED, "q / q_out rows must be 16-byte aligned with strides >= heads * head_dim, % 8");
+    vecs = step->rows * heads * (d / 8) / 256 + 1;
+  }
+  if (!paged_grid_ok(*cache, *step, vecs)) return fail(EE_ERR_UNSUPPORTED, "too many rows in one step");
+  return check_launch(ee::launch_paged_append(paged_args(*cache), paged_step_args(*step),
+                                              {static_cast<const __half*>(k), ldk}, {static_cast<const __half*>(v), ldv},
+                                              static_cast<const __half*>(cos), static_cast<const __half*>(sin), ld_cs,
+                                              {static_cast<const __half*>(q), ldq}, static_cast<int>(heads),
+                                              static_cast<__half*>(q_out), ldqo, as_stream(stream)),
+                      "paged_append");
+}
+
+int ee_paged_read(const ee_paged_cache* cache, const ee_paged_step* step, void* k, int64_t ldk, void* v, int64_t ldv,
+                  void* stream) {
+  int st = paged_cache_ok(cache);
+  if (st == EE_OK) st = paged_step_ok(step);
+  if (st != EE_OK) return st;
+  if (step->batch == 0 || step->rows == 0) return EE_OK;
+  if (!k || !v) return fail(EE_ERR_INVALID, "k and v are required");
+  const int64_t row = cache->kv_heads * cache->head_dim;
+  if (!rows_ok(k, ldk, row) || !rows_ok(v, ldv, row))
+    return fail(EE_ERR_MISALIGNED, "K / V rows must be 16-byte aligned with strides >= kv_heads * head_dim, % 8");
+  if (!paged_grid_ok(*cache, *step, 0)) return fail(EE_ERR_UNSUPPORTED, "too many rows in one step");
+  return check_launch(ee::launch_paged_read(paged_args(*cache), paged_step_args(*step), static_cast<__half*>(k), ldk,
+                                            static_cast<__half*>(v), ldv, as_stream(stream)),
+                      "paged_read");
+}
+
+size_t ee_paged_workspace_bytes(const ee_paged_cache* cache) {
+  if (cache == nullptr || (cache->head_dim != 64 && cache->head_dim != 128)) return 0;
+  return align256(ee::paged_workspace_bytes(cache->head_dim));
+}
+size_t ee_paged_workspace_head_bytes(void) { return ee::paged_head_bytes(); }
+
+int ee_paged_attention(const ee_paged_cache* cache, const ee_paged_step* step, const void* q, int64_t ldq, int64_t heads,
+                       float scale, void* out, int64_t ldo, float* H, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  int st = paged_cache_ok(cache);
+  if (st == EE_OK) st = paged_step_ok(step);
+  if (st != EE_OK) return st;
+  if (heads <= 0 || heads % cache->kv_heads || heads > 65536)
+    return fail(EE_ERR_UNSUPPORTED, "heads must be a multiple of kv_heads, at most 65536");
+  if (!(scale > 0.f) || scale > 3e38f) return fail(EE_ERR_INVALID, "scale must be positive and finite");
+  if (step->batch == 0 || step->rows == 0) return EE_OK;
+  if (!q || !out) return fail(EE_ERR_INVALID, "q and out are required");
+  const int64_t d = cache->head_dim;
+  if (!rows_ok(q, ldq, heads * d) || !rows_ok(out, ldo, heads * d) || (reinterpret_cast<uintptr_t>(H) & 3u))
+    return fail(EE_ERR_MISALIGNED, "q / out rows 16-byte aligned with strides >= heads * head_dim, % 8; H 4-byte aligned");
+  st = check_ws(workspace, workspace_bytes, ee_paged_workspace_bytes(cache));
+  if (st != EE_OK) return st;
+  return check_launch(ee::launch_paged_attention(paged_args(*cache), paged_step_args(*step),
+                                                 {static_cast<const __half*>(q), ldq}, static_cast<int>(heads),
+                                                 step->max_new, scale, static_cast<__half*>(out), ldo, H, workspace,
+                                                 as_stream(stream)),
+                      "paged_attention");
 }
 
 int ee_head_mean_entropy(const float* H, int64_t B, int64_t Hq, int64_t S, float* token_entropy,

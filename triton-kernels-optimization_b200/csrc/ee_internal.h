@@ -18,6 +18,7 @@ enum DeviceError : int {
   kErrTmem = 2,         // tensor-memory allocation returned an unusable address
   kErrShape = 4,        // a bucket holds more rows than the kernel's tile was launched for
   kErrCapacity = 8,     // a KV-cache pool or sequence was full: the token was not stored
+  kErrPage = 16,        // a paged step names a sequence, page or position that the cache does not have
 };
 
 // ----------------------------------------------------------------- row kernels
@@ -175,6 +176,34 @@ int launch_kv_append(const KvCacheArgs& c, const void* k_rows, int64_t ldk, cons
 int launch_kv_decode_attention(const KvCacheArgs& c, const void* q, int64_t ldq, int64_t Hq, const void* k_new,
                                const void* v_new, int64_t ld_new, float scale, int splits, float* part, void* out,
                                int64_t ldo, float* H, cudaStream_t s);
+// paged KV cache (ee_paged.cuh); the fields of ee_paged_cache / ee_paged_step (include/ee_b200.h)
+struct PagedArgs {
+  int64_t num_pages, kv_heads, head_dim, page_size, max_seqs, max_pages;
+  int tier, page_shift;  // Bucket; log2 page_size
+  uint8_t* pages;        // [num_pages, kv_heads, 2 (K, V), page_size x head_dim]
+  float* scale;          // [num_pages, kv_heads, 2], 8-bit tiers
+  __half* open;          // [max_seqs, 2, kv_heads, 2, page_size x head_dim], 8-bit tiers
+  int32_t* table;        // [max_seqs, max_pages]
+};
+struct PagedStepArgs {
+  int64_t batch, rows;
+  const int32_t *seq, *start, *length, *cu;  // [batch], [batch], [batch], [batch + 1]
+};
+struct PagedRows {
+  const __half* p;  // [rows, heads * head_dim], row stride ld elements
+  int64_t ld;
+};
+int launch_paged_append(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& k, const PagedRows& v,
+                        const __half* cos, const __half* sin, int64_t ld_cs, const PagedRows& q, int heads, __half* q_out,
+                        int64_t ldqo, cudaStream_t s);
+int launch_paged_read(const PagedArgs& c, const PagedStepArgs& st, __half* k, int64_t ldk, __half* v, int64_t ldv,
+                      cudaStream_t s);
+int launch_paged_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new,
+                           float scale, __half* out, int64_t ldo, float* H, void* workspace, cudaStream_t s);
+size_t paged_head_bytes();                   // zeroed once by the owner of a workspace
+size_t paged_workspace_bytes(int64_t D);
+int read_and_clear_paged_error(int* value);
+
 // flash attention with row entropy (ee_attention.cuh): Q [B*Hq*S, D], K [B*Hkv*S, D],
 // V^T [B*Hkv*D, S_pad] maps (box 64 x 128 / 64 x D), outputs O [B, S, Hq, D], H [B, Hq, S]
 constexpr int kAttnTile = 128;  // queries per attention CTA and keys per KV tile

@@ -1,0 +1,145 @@
+// ee_paged.cu - device translation unit of the paged KV cache: its kernels (ee_paged.cuh) and
+// the launchers the C-ABI layer calls.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+#include <utility>
+
+#include "ee_paged.cuh"
+
+namespace ee {
+
+int sm_count();  // ee_kernels.cu
+
+namespace {
+inline int status_of(cudaError_t e) { return e == cudaSuccess ? 0 : -4; }
+
+// Launch with programmatic stream serialization (griddep_wait in the kernel).
+template <typename... KArgs, typename... Args>
+int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return status_of(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// dynamic shared memory above 48 KB, set once per device and kernel
+template <auto kKernel>
+int allow_smem(size_t bytes) {
+  static std::once_flag once[64];
+  static cudaError_t err[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -4;
+  std::call_once(once[dev], [&] {
+    err[dev] = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  });
+  return status_of(err[dev]);
+}
+
+int64_t block_slots(const PagedArgs& c, const PagedStepArgs& st) { return (st.rows >> c.page_shift) + 2 * st.batch; }
+
+template <int D, int TIER>
+int run_append(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& k, const PagedRows& v, const __half* cos,
+               const __half* sin, int64_t ld_cs, const PagedRows& q, int heads, __half* q_out, int64_t ldqo,
+               cudaStream_t s) {
+  int e = allow_smem<paged_append_kernel<D, TIER>>(paged_stage_bytes(128, D));
+  if (e != 0) return e;
+  const int64_t kv = block_slots(c, st) * c.kv_heads;
+  const int64_t qn = q.p == nullptr ? 0 : (st.rows * heads * (D / 16) + kPagedAppendThreads - 1) / kPagedAppendThreads;
+  return launch_pdl(paged_append_kernel<D, TIER>, dim3(static_cast<unsigned>(kv + qn)), dim3(kPagedAppendThreads),
+                    paged_stage_bytes(static_cast<int>(c.page_size), D), s, c, st, k, v, cos, sin, ld_cs, q, heads, q_out,
+                    ldqo, kv);
+}
+template <int D, int TIER>
+int run_read(const PagedArgs& c, const PagedStepArgs& st, __half* k, int64_t ldk, __half* v, int64_t ldv, cudaStream_t s) {
+  int e = allow_smem<paged_read_kernel<D, TIER>>(paged_stage_bytes(128, D));
+  if (e != 0) return e;
+  return launch_pdl(paged_read_kernel<D, TIER>, dim3(static_cast<unsigned>(block_slots(c, st) * c.kv_heads)), dim3(kPagedAppendThreads),
+                    paged_stage_bytes(static_cast<int>(c.page_size), D), s, c, st, k, ldk, v, ldv);
+}
+
+// CTAs per SM of the few-row kernel, by its launch bounds
+constexpr int few_ctas(int nb) { return nb == 1 ? 3 : 2; }
+
+template <int D, int TIER, int NB>
+int run_few(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, const PagedRows& q, int heads, float scale,
+            __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
+  // no CTA for less than four turns of its warps: shorter parts cost more in joining than
+  // they save
+  return launch_pdl(paged_attention_kernel<D, TIER, NB>, dim3(static_cast<unsigned>(sm_count() * few_ctas(NB))),
+                    dim3(kFewThreads), 0, s, c, st, pl, q, heads, scale, out, ldo, H, tickets, part,
+                    int64_t(4 * kFewTile));
+}
+template <int D, int TIER>
+int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new, float scale,
+                  __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
+  const int G = heads / static_cast<int>(c.kv_heads);
+  const bool one = G * max_new <= 8;
+  PagedPlan pl;
+  const int R = one ? 8 : 16;
+  pl.G = G;
+  pl.hgroups = (G + R - 1) / R;
+  pl.Gc = (G + pl.hgroups - 1) / pl.hgroups;
+  pl.TQ = R / pl.Gc;
+  if (one) return run_few<D, TIER, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  return run_few<D, TIER, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+}
+}  // namespace
+
+size_t paged_head_bytes() { return 4096; }  // a ticket per CTA
+size_t paged_workspace_bytes(int64_t D) {
+  return paged_head_bytes() + size_t(2) * sm_count() * few_ctas(1) * 16 * (D + 4) * sizeof(float);
+}
+
+#define EE_PAGED_DISPATCH(call)                                            \
+  (c.head_dim == 64 ? (c.tier == kINT8  ? call<64, kINT8> PAGED_ARGS       \
+                       : c.tier == kFP8 ? call<64, kFP8> PAGED_ARGS        \
+                                        : call<64, kFP16> PAGED_ARGS)      \
+                    : (c.tier == kINT8  ? call<128, kINT8> PAGED_ARGS      \
+                       : c.tier == kFP8 ? call<128, kFP8> PAGED_ARGS       \
+                                        : call<128, kFP16> PAGED_ARGS))
+
+int launch_paged_append(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& k, const PagedRows& v,
+                        const __half* cos, const __half* sin, int64_t ld_cs, const PagedRows& q, int heads, __half* q_out,
+                        int64_t ldqo, cudaStream_t s) {
+#define PAGED_ARGS (c, st, k, v, cos, sin, ld_cs, q, heads, q_out, ldqo, s)
+  return EE_PAGED_DISPATCH(run_append);
+#undef PAGED_ARGS
+}
+int launch_paged_read(const PagedArgs& c, const PagedStepArgs& st, __half* k, int64_t ldk, __half* v, int64_t ldv,
+                      cudaStream_t s) {
+#define PAGED_ARGS (c, st, k, ldk, v, ldv, s)
+  return EE_PAGED_DISPATCH(run_read);
+#undef PAGED_ARGS
+}
+int launch_paged_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new,
+                           float scale, __half* out, int64_t ldo, float* H, void* workspace, cudaStream_t s) {
+  uint32_t* tickets = static_cast<uint32_t*>(workspace);
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + paged_head_bytes());
+#define PAGED_ARGS (c, st, q, heads, max_new, scale, out, ldo, H, tickets, part, s)
+  return EE_PAGED_DISPATCH(run_attention);
+#undef PAGED_ARGS
+}
+
+int read_and_clear_paged_error(int* value) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_paged_error, sizeof(int));
+  if (e != cudaSuccess) return -4;
+  if (v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_paged_error, &zero, sizeof(int));
+    if (e != cudaSuccess) return -4;
+  }
+  *value = v;
+  return 0;
+}
+
+}  // namespace ee

@@ -1,0 +1,1032 @@
+// ee_paged.cuh - paged KV cache: sequences of different lengths keep their keys and values in
+// pages of P tokens (16 .. 128) handed out one by one, in fp16 or in 8 bits with one scale
+// for each page and KV head (K and V apart).
+//   * paged_append_kernel: a step's new tokens: rotary embedding of q and k on the way, the
+//     rows into their pages; a block of P tokens is quantised once, when it is complete;
+//   * paged_attention_kernel: the step's query rows against everything cached, a few rows per
+//     (sequence, KV head) at a time, with the entropy of every softmax row;
+//   * paged_read_kernel: rows of a span back as fp16.
+//
+// Blocks.  Tokens jP .. jP + P - 1 of a sequence are block j; table[seq][j] is its page.  In
+// an 8-bit tier a block is quantised when its last token arrives: s = max |x| / 127 (int8) or
+// / 448 (e4m3) over its P x D values of a head, code = rn(x / s) (IEEE
+// divisions: the codes are the same on every path that computes them).  Until then its tokens are in the sequence's
+// open buffer in fp16, slot j & 1; the block before it keeps its fp16 rows in the other slot.  So
+// the cache's contents depend on the tokens alone, not on how they were cut into appends, and
+// up to P tokens can be taken back exactly.  The fp16 tier writes tokens into their pages.
+//
+// Order inside a page.  Tokens go in groups of 16, and a group's values lie in the order in
+// which a warp's lanes hold the operand of a 16 x 8 x 16 MMA: 16 bytes of lane 0, of lane 1, ..
+// (lane = 4 gq + q4), so every read is a full line and no value moves between lanes:
+//   K  lane (gq, q4) holds tokens gq and gq + 8, dimensions q4 D/4 .. + D/4 - 1;
+//   V  lane (gq, q4) holds tokens 2 q4, 2 q4 + 1, 2 q4 + 8, 2 q4 + 9, dimensions gq D/8 ..,
+//      the two tokens of a pair side by side.
+// int8 codes are kept plus 128: 0x64 above such a byte is the fp16 number 1024 + byte.
+//
+// Included once, by ee_paged.cu.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "ee_internal.h"
+#include "ee_ptx.cuh"
+
+namespace ee {
+
+__device__ int g_paged_error = 0;  // the paged kernels' error word (DeviceError bits)
+
+// ----------------------------------------------------------------------------------
+// order inside a page (elements from the start of the head's K or V part)
+// ----------------------------------------------------------------------------------
+template <int D, bool kWide>  // kWide: fp16 elements, else 8-bit
+__device__ __forceinline__ int page_k_offset(int t, int d) {
+  constexpr int E = kWide ? 8 : 16;  // elements per 16 bytes
+  const int q4 = d / (D / 4), r = d % (D / 4);
+  const int piece = r / E;
+  const int lane = (t & 7) * 4 + q4;
+  return (t >> 4) * 16 * D + ((((t >> 3) & 1) * (D / 4 / E) + piece) * 32 + lane) * E + r % E;
+}
+template <int D, bool kWide>
+__device__ __forceinline__ int page_v_offset(int t, int d) {
+  const int gq = d / (D / 8), r = d % (D / 8), mb = r >> 1, j = r & 1;
+  const int th = (t >> 3) & 1, lane = gq * 4 + ((t & 7) >> 1), lo = t & 1;
+  if constexpr (kWide) return (t >> 4) * 16 * D + (mb * 32 + lane) * 8 + (th * 2 + j) * 2 + lo;
+  return (t >> 4) * 16 * D + ((mb >> 1) * 32 + lane) * 16 + (mb & 1) * 8 + th * 4 + j * 2 + lo;
+}
+
+__device__ __forceinline__ uint8_t* paged_block(const PagedArgs& c, int64_t page, int64_t h, int which) {
+  const int64_t bytes = c.page_size * c.head_dim * (c.tier == kFP16 ? 2 : 1);
+  return c.pages + ((page * c.kv_heads + h) * 2 + which) * bytes;
+}
+__device__ __forceinline__ __half* paged_open(const PagedArgs& c, int64_t seq, int64_t blk, int64_t h, int which) {
+  return c.open + (((seq * 2 + (blk & 1)) * c.kv_heads + h) * 2 + which) * c.page_size * c.head_dim;
+}
+// page of block blk, or -1 (outside the table, not handed out, outside the pool)
+__device__ __forceinline__ int paged_page(const PagedArgs& c, int64_t seq, int64_t blk) {
+  if (blk >= c.max_pages) return -1;
+  const int p = c.table[seq * c.max_pages + blk];
+  return p >= 0 && p < c.num_pages ? p : -1;
+}
+
+// one sequence of a step, checked against the cache; ok == false: nothing of it is touched
+struct PagedSeq {
+  int64_t seq, start, n, length, row0;
+  bool ok;
+};
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& c, const PagedStepArgs& st, int64_t b) {
+  PagedSeq s;
+  s.seq = st.seq[b];
+  s.start = st.start[b];
+  s.length = st.length[b];
+  s.row0 = st.cu[b];
+  s.n = static_cast<int64_t>(st.cu[b + 1]) - s.row0;
+  s.ok = s.seq >= 0 && s.seq < c.max_seqs && s.start >= 0 && s.row0 >= 0 && s.n >= 0 && s.row0 + s.n <= st.rows &&
+         s.start + s.n <= s.length && s.length <= c.max_pages * c.page_size;
+  return s;
+}
+
+// Work slots of a step's blocks: sequence b has the slots cu[b] / P + 2 b .. , two more than
+// whole blocks fit its rows, which is enough wherever the first block begins.  The sequence
+// of a slot by a 32-way search over the warp's lanes.
+__device__ __forceinline__ int64_t paged_slot_base(const PagedStepArgs& st, int64_t b, int shift) {
+  return (static_cast<int64_t>(st.cu[b]) >> shift) + 2 * b;
+}
+__device__ __forceinline__ int64_t paged_slot_seq(const PagedStepArgs& st, int64_t slot, int shift, int lane) {
+  int64_t lo = 0, n = st.batch;  // the answer is in [lo, lo + n)
+  while (n > 1) {
+    const int64_t step = (n + 31) / 32;
+    const int64_t b = lo + lane * step;
+    const bool le = b < lo + n && (lane == 0 || paged_slot_base(st, b, shift) <= slot);
+    const unsigned m = __ballot_sync(0xffffffffu, le);
+    const int k = 31 - __clz(m);
+    const int64_t at = lo + k * step, end = lo + n;
+    lo = at;
+    n = at + step < end ? step : end - at;
+  }
+  return lo;
+}
+
+// ----------------------------------------------------------------------------------
+// append
+// ----------------------------------------------------------------------------------
+// eight values of a row rotated: y_j = x_j cos_j + rot_j sin_j, rot = (-x[D/2 ..], x[.. D/2]).
+// fp32 with one rounding to fp16 at the end.
+__device__ __forceinline__ uint4 rope8(const uint4& x, const uint4& partner, bool low_half, const uint4& c,
+                                       const uint4& sn) {
+  const __half2* hx = reinterpret_cast<const __half2*>(&x);
+  const __half2* hp = reinterpret_cast<const __half2*>(&partner);
+  const __half2* hc = reinterpret_cast<const __half2*>(&c);
+  const __half2* hs = reinterpret_cast<const __half2*>(&sn);
+  uint4 o;
+  __half2* ho = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 fx = __half22float2(hx[k]), fc = __half22float2(hc[k]), fs = __half22float2(hs[k]);
+    float2 fp = __half22float2(hp[k]);
+    if (low_half) fp = make_float2(-fp.x, -fp.y);
+    ho[k] = __floats2half2_rn(fmaf(fp.x, fs.x, fx.x * fc.x), fmaf(fp.y, fs.y, fx.y * fc.y));
+  }
+  return o;
+}
+template <int D>
+__device__ __forceinline__ uint4 load_rotated(const __half* row, int d0, const __half* cs, const __half* sn) {
+  const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
+  if (cs == nullptr) return x;
+  const bool low = d0 < D / 2;
+  const uint4 p = *reinterpret_cast<const uint4*>(row + (low ? d0 + D / 2 : d0 - D / 2));
+  return rope8(x, p, low, *reinterpret_cast<const uint4*>(cs + d0), *reinterpret_cast<const uint4*>(sn + d0));
+}
+
+constexpr int kPagedAppendThreads = 256;
+// shared memory of an append CTA: the block's K and V rows, padded by 16 bytes
+__host__ __device__ constexpr size_t paged_stage_bytes(int page, int D) { return size_t(2) * page * (D + 8) * 2; }
+
+// One CTA per (touched block, KV head), then CTAs that rotate q (kPagedAppendThreads pairs of
+// eight values each).
+template <int D, int TIER>
+__global__ void __launch_bounds__(kPagedAppendThreads)
+    paged_append_kernel(const PagedArgs c, const PagedStepArgs st, const PagedRows k, const PagedRows v,
+                        const __half* __restrict__ cos, const __half* __restrict__ sin, int64_t ld_cs,
+                        const PagedRows q, int heads, __half* q_out, int64_t ldqo, int64_t kv_ctas) {
+  constexpr int VPR = D / 8;    // 16-byte vectors per row and head
+  constexpr int LD = D + 8;     // stage row, halves
+  extern __shared__ __align__(16) uint8_t paged_smem[];
+  __shared__ float s_max[2][kPagedAppendThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  griddep_wait();
+  griddep_launch_dependents();
+  if (blockIdx.x >= kv_ctas) {  // q: a thread has both halves of its pairs, so q_out may be q
+    const int64_t i = (blockIdx.x - kv_ctas) * kPagedAppendThreads + tid;
+    const int64_t row = i / (heads * (VPR / 2));
+    if (row >= st.rows) return;
+    const int vec = static_cast<int>(i % (heads * (VPR / 2)));
+    const int h = vec / (VPR / 2), d0 = (vec % (VPR / 2)) * 8, d1 = d0 + D / 2;
+    const __half* src = q.p + row * q.ld + h * D;
+    uint4 lo = *reinterpret_cast<const uint4*>(src + d0), hi = *reinterpret_cast<const uint4*>(src + d1);
+    if (cos != nullptr) {
+      const __half* cr = cos + row * ld_cs;
+      const __half* sr = sin + row * ld_cs;
+      const uint4 x = rope8(lo, hi, true, *reinterpret_cast<const uint4*>(cr + d0), *reinterpret_cast<const uint4*>(sr + d0));
+      hi = rope8(hi, lo, false, *reinterpret_cast<const uint4*>(cr + d1), *reinterpret_cast<const uint4*>(sr + d1));
+      lo = x;
+    }
+    __half* dst = q_out + row * ldqo + h * D;
+    *reinterpret_cast<uint4*>(dst + d0) = lo;
+    *reinterpret_cast<uint4*>(dst + d1) = hi;
+    return;
+  }
+  const int64_t slot = blockIdx.x / c.kv_heads;
+  const int h = static_cast<int>(blockIdx.x % c.kv_heads);
+  const int64_t b = paged_slot_seq(st, slot, c.page_shift, lane);
+  const PagedSeq s = paged_seq(c, st, b);
+  const int64_t P = c.page_size;
+  if (!s.ok) {
+    if (tid == 0) atomicOr(&g_paged_error, kErrPage);
+    return;
+  }
+  const int64_t blk0 = s.start >> c.page_shift, blk = blk0 + slot - paged_slot_base(st, b, c.page_shift);
+  const int64_t end = s.start + s.n, p0 = blk << c.page_shift;
+  if (s.n == 0 || p0 >= end) return;
+  const int64_t blkN = (end - 1) >> c.page_shift;
+  const int t0 = static_cast<int>(s.start > p0 ? s.start - p0 : 0);                // new tokens of the block: [t0, t1)
+  const int t1 = static_cast<int>(end - p0 < P ? end - p0 : P);
+  const int page = paged_page(c, s.seq, blk);
+  if (page < 0 && tid == 0) atomicOr(&g_paged_error, kErrPage);
+  __half* sk = reinterpret_cast<__half*>(paged_smem);
+  __half* sv = sk + P * LD;
+
+  // rows [r0, r1) of block x (new tokens) into the stage
+  auto stage_new = [&](int64_t base, int r0, int r1) {
+    for (int i = tid; i < (r1 - r0) * VPR; i += kPagedAppendThreads) {
+      const int t = r0 + i / VPR, d0 = (i % VPR) * 8;
+      const int64_t row = s.row0 + base + t - s.start;
+      *reinterpret_cast<uint4*>(sk + t * LD + d0) =
+          load_rotated<D>(k.p + row * k.ld + h * D, d0, cos == nullptr ? nullptr : cos + row * ld_cs, sin + row * ld_cs);
+      *reinterpret_cast<uint4*>(sv + t * LD + d0) = *reinterpret_cast<const uint4*>(v.p + row * v.ld + h * D + d0);
+    }
+  };
+  // stage rows [r0, r1) to fp16 in page order at kd / vd
+  auto store_wide = [&](__half* kd, __half* vd, int r0, int r1) {
+    for (int i = tid; i < (r1 - r0) * VPR; i += kPagedAppendThreads) {
+      const int t = r0 + i / VPR, d0 = (i % VPR) * 8;
+      *reinterpret_cast<uint4*>(kd + page_k_offset<D, true>(t, d0)) = *reinterpret_cast<const uint4*>(sk + t * LD + d0);
+    }
+    const int g0 = r0 >> 4, g1 = (r1 + 15) >> 4;
+    for (int i = tid; i < (g1 - g0) * 2 * D; i += kPagedAppendThreads) {  // 16-byte units of V
+      const int g = g0 + i / (2 * D), u = i % (2 * D);
+      const int mb = u >> 5, ln = u & 31, gq = ln >> 2, q4 = ln & 3;
+      const int d0 = gq * (D / 8) + 2 * mb, t = 16 * g + 2 * q4;
+      __half val[8];
+      bool all = true;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int tt = t + (e >> 2) * 8 + (e & 1);
+        const bool in = tt >= r0 && tt < r1;
+        all = all && in;
+        val[e] = in ? sv[tt * LD + d0 + ((e >> 1) & 1)] : __half(0.f);
+      }
+      __half* dst = vd + g * 16 * D + u * 8;
+      if (all) {
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(val);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int tt = t + (e >> 2) * 8 + (e & 1);
+          if (tt >= r0 && tt < r1) dst[e] = val[e];
+        }
+      }
+    }
+  };
+
+  stage_new(p0, t0, t1);
+  if constexpr (TIER == kFP16) {
+    __syncthreads();
+    if (page >= 0)
+      store_wide(reinterpret_cast<__half*>(paged_block(c, page, h, 0)),
+                 reinterpret_cast<__half*>(paged_block(c, page, h, 1)), t0, t1);
+    return;
+  } else {
+    const bool complete = t1 == P;
+    if (complete && t0 > 0) {  // the block's earlier tokens, from the open buffer
+      const __half* ko = paged_open(c, s.seq, blk, h, 0);
+      const __half* vo = paged_open(c, s.seq, blk, h, 1);
+      for (int i = tid; i < t0 * VPR; i += kPagedAppendThreads) {
+        const int t = i / VPR, d0 = (i % VPR) * 8;
+        *reinterpret_cast<uint4*>(sk + t * LD + d0) = *reinterpret_cast<const uint4*>(ko + page_k_offset<D, true>(t, d0));
+      }
+      for (int i = tid; i < ((t0 + 15) >> 4) * 2 * D; i += kPagedAppendThreads) {
+        const int g = i / (2 * D), u = i % (2 * D);
+        const int mb = u >> 5, ln = u & 31, gq = ln >> 2, q4 = ln & 3;
+        const int d0 = gq * (D / 8) + 2 * mb, t = 16 * g + 2 * q4;
+        const uint4 x = *reinterpret_cast<const uint4*>(vo + g * 16 * D + u * 8);
+        const __half* val = reinterpret_cast<const __half*>(&x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int tt = t + (e >> 2) * 8 + (e & 1);
+          if (tt < t0) sv[tt * LD + d0 + ((e >> 1) & 1)] = val[e];
+        }
+      }
+    }
+    __syncthreads();
+    if (complete && page >= 0) {
+      float mk = 0.f, mv = 0.f;
+      bool bad_k = false, bad_v = false;  // fmaxf drops NaN: carried apart
+      for (int i = tid; i < static_cast<int>(P) * VPR; i += kPagedAppendThreads) {
+        const int o = (i / VPR) * LD + (i % VPR) * 8;
+        const uint4 xk = *reinterpret_cast<const uint4*>(sk + o), xv = *reinterpret_cast<const uint4*>(sv + o);
+        const __half2* a = reinterpret_cast<const __half2*>(&xk);
+        const __half2* w = reinterpret_cast<const __half2*>(&xv);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 fa = __half22float2(a[e]), fw = __half22float2(w[e]);
+          mk = fmaxf(mk, fmaxf(fabsf(fa.x), fabsf(fa.y)));
+          mv = fmaxf(mv, fmaxf(fabsf(fw.x), fabsf(fw.y)));
+          bad_k = bad_k || fa.x != fa.x || fa.y != fa.y;
+          bad_v = bad_v || fw.x != fw.x || fw.y != fw.y;
+        }
+      }
+      if (bad_k) mk = __builtin_huge_valf();  // a NaN makes the block's scale infinite, and its rows NaN
+      if (bad_v) mv = __builtin_huge_valf();
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        mk = fmaxf(mk, __shfl_xor_sync(0xffffffffu, mk, o));
+        mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+      }
+      if (lane == 0) {
+        s_max[0][warp] = mk;
+        s_max[1][warp] = mv;
+      }
+      __syncthreads();
+      mk = s_max[0][0];
+      mv = s_max[1][0];
+#pragma unroll
+      for (int w = 1; w < kPagedAppendThreads / 32; ++w) {
+        mk = fmaxf(mk, s_max[0][w]);
+        mv = fmaxf(mv, s_max[1][w]);
+      }
+      constexpr float kTop = TIER == kINT8 ? 127.f : 448.f;
+      const float ks = __fdiv_rn(mk, kTop), vs = __fdiv_rn(mv, kTop);
+      if (tid == 0) *reinterpret_cast<float2*>(c.scale + (static_cast<int64_t>(page) * c.kv_heads + h) * 2) = make_float2(ks, vs);
+      const float dk = ks > 0.f ? ks : 1.f, dv = vs > 0.f ? vs : 1.f;  // an all-zero block: scale 0, codes 0
+      auto code2 = [&](float a, float w) -> uint32_t {  // two codes, low byte first
+        if constexpr (TIER == kINT8) {
+          const int ia = __float2int_rn(fminf(fmaxf(a, -127.f), 127.f)), iw = __float2int_rn(fminf(fmaxf(w, -127.f), 127.f));
+          return static_cast<uint32_t>(ia + 128) | static_cast<uint32_t>(iw + 128) << 8;
+        } else {
+          uint16_t o;
+          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(w), "f"(a));
+          return o;
+        }
+      };
+      uint8_t* kd = paged_block(c, page, h, 0);
+      uint8_t* vd = paged_block(c, page, h, 1);
+      const int units = static_cast<int>(P) * D / 16;
+      for (int i = tid; i < units; i += kPagedAppendThreads) {
+        const int g = i / D, u = i % D;  // D units per group of 16 tokens
+        const int ln = u & 31, gq = ln >> 2, q4 = ln & 3;
+        {  // K: 16 dimensions of one token
+          const int half = u / 32 / (D / 64), piece = u / 32 % (D / 64);
+          const __half* src = sk + (16 * g + 8 * half + gq) * LD + q4 * (D / 4) + piece * 16;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = __half22float2(reinterpret_cast<const __half2*>(src)[2 * e]);
+            const float2 z = __half22float2(reinterpret_cast<const __half2*>(src)[2 * e + 1]);
+            w[e] = code2(__fdiv_rn(a.x, dk), __fdiv_rn(a.y, dk)) | code2(__fdiv_rn(z.x, dk), __fdiv_rn(z.y, dk)) << 16;
+          }
+          *reinterpret_cast<uint4*>(kd + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        {  // V: four dimensions of four tokens
+          const int d0 = gq * (D / 8) + 4 * (u >> 5);
+          const __half* src = sv + (16 * g + 2 * q4) * LD + d0;
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // word: mb = e >> 1, th = e & 1
+            const __half* x = src + (e & 1) * 8 * LD + (e >> 1) * 2;
+            w[e] = code2(__fdiv_rn(__half2float(x[0]), dv), __fdiv_rn(__half2float(x[LD]), dv)) |
+                   code2(__fdiv_rn(__half2float(x[1]), dv), __fdiv_rn(__half2float(x[LD + 1]), dv)) << 16;
+          }
+          *reinterpret_cast<uint4*>(vd + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+    // the fp16 rows of the sequence's last two blocks.  A later block whose slot holds the
+    // tokens that the first block has yet to read is written by the first block's CTA, after
+    // it read them.
+    const bool first_reads = (s.start & (P - 1)) != 0 && blk0 < blkN;
+    if (blk >= blkN - 1 && !(first_reads && blk > blk0 && ((blk - blk0) & 1) == 0))
+      store_wide(paged_open(c, s.seq, blk, h, 0), paged_open(c, s.seq, blk, h, 1), t0, t1);
+    if (first_reads && blk == blk0) {
+      for (int64_t later = blkN - 1 > blk0 ? blkN - 1 : blkN; later <= blkN; ++later) {
+        if (later == blk0 || ((later - blk0) & 1) != 0) continue;
+        __syncthreads();
+        const int r1 = static_cast<int>(end - (later << c.page_shift) < P ? end - (later << c.page_shift) : P);
+        stage_new(later << c.page_shift, 0, r1);
+        __syncthreads();
+        store_wide(paged_open(c, s.seq, later, h, 0), paged_open(c, s.seq, later, h, 1), 0, r1);
+      }
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// read back
+// ----------------------------------------------------------------------------------
+// int8 codes (plus 128) of one word -> two fp16 pairs, exactly
+__device__ __forceinline__ void u8x4_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140);  // bytes w0, 0x64, w1, 0x64
+  const uint32_t b = __byte_perm(w, 0x64646464u, 0x4342);  // bytes w2, 0x64, w3, 0x64
+  const __half2 off = __halves2half2(__ushort_as_half(0x6480u), __ushort_as_half(0x6480u));  // 1152
+  const __half2 ra = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+  const __half2 rb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+  lo = *reinterpret_cast<const uint32_t*>(&ra);
+  hi = *reinterpret_cast<const uint32_t*>(&rb);
+}
+__device__ __forceinline__ void f8x4_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
+template <int TIER>
+__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (TIER == kINT8) u8x4_to_h2(w, lo, hi);
+  else f8x4_to_h2(w, lo, hi);
+}
+
+// One CTA per (touched block, KV head): the block's rows in the span, staged in shared memory
+// in token order, to k_out / v_out.
+template <int D, int TIER>
+__global__ void __launch_bounds__(kPagedAppendThreads)
+    paged_read_kernel(const PagedArgs c, const PagedStepArgs st, __half* __restrict__ k_out, int64_t ldk,
+                      __half* __restrict__ v_out, int64_t ldv) {
+  constexpr int VPR = D / 8;
+  constexpr int LD = D + 8;
+  extern __shared__ __align__(16) uint8_t paged_smem[];
+  const int tid = threadIdx.x, lane = tid & 31;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t slot = blockIdx.x / c.kv_heads;
+  const int h = static_cast<int>(blockIdx.x % c.kv_heads);
+  const int64_t b = paged_slot_seq(st, slot, c.page_shift, lane);
+  const PagedSeq s = paged_seq(c, st, b);
+  const int64_t P = c.page_size;
+  if (!s.ok) {
+    if (tid == 0) atomicOr(&g_paged_error, kErrPage);
+    return;
+  }
+  const int64_t blk = (s.start >> c.page_shift) + slot - paged_slot_base(st, b, c.page_shift);
+  const int64_t end = s.start + s.n, p0 = blk << c.page_shift;
+  if (s.n == 0 || p0 >= end) return;
+  const int t0 = static_cast<int>(s.start > p0 ? s.start - p0 : 0);
+  const int t1 = static_cast<int>(end - p0 < P ? end - p0 : P);
+  __half* sk = reinterpret_cast<__half*>(paged_smem);
+  __half* sv = sk + P * LD;
+  const bool open = TIER != kFP16 && p0 + P > s.length;
+  const int page = open ? 0 : paged_page(c, s.seq, blk);
+  if (page < 0) {  // a hole: zeros, and the error word
+    if (tid == 0) atomicOr(&g_paged_error, kErrPage);
+    for (int i = tid; i < static_cast<int>(P) * LD / 4; i += kPagedAppendThreads)
+      reinterpret_cast<uint4*>(paged_smem)[i] = make_uint4(0, 0, 0, 0);
+  } else if (TIER == kFP16 || open) {
+    const __half* kp = open ? paged_open(c, s.seq, blk, h, 0) : reinterpret_cast<const __half*>(paged_block(c, page, h, 0));
+    const __half* vp = open ? paged_open(c, s.seq, blk, h, 1) : reinterpret_cast<const __half*>(paged_block(c, page, h, 1));
+    const int g0 = t0 >> 4, g1 = (t1 + 15) >> 4;
+    for (int i = tid; i < (g1 - g0) * 2 * D; i += kPagedAppendThreads) {
+      const int g = g0 + i / (2 * D), u = i % (2 * D);
+      const int ln = u & 31, gq = ln >> 2, q4 = ln & 3, piece = u >> 5;
+      const uint4 xk = *reinterpret_cast<const uint4*>(kp + g * 16 * D + u * 8);
+      const uint4 xv = *reinterpret_cast<const uint4*>(vp + g * 16 * D + u * 8);
+      const int half = piece / (D / 32), kp8 = piece % (D / 32);
+      *reinterpret_cast<uint4*>(sk + (16 * g + 8 * half + gq) * LD + q4 * (D / 4) + kp8 * 8) = xk;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&xv);
+      __half* dst = sv + (16 * g + 2 * q4) * LD + gq * (D / 8) + 2 * piece;
+#pragma unroll
+      for (int th = 0; th < 2; ++th) {
+        *reinterpret_cast<uint32_t*>(dst + th * 8 * LD) = __byte_perm(w[2 * th], w[2 * th + 1], 0x5410);
+        *reinterpret_cast<uint32_t*>(dst + (th * 8 + 1) * LD) = __byte_perm(w[2 * th], w[2 * th + 1], 0x7632);
+      }
+    }
+  } else {
+    const float2 sc = *reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(page) * c.kv_heads + h) * 2);
+    const uint8_t* kp = paged_block(c, page, h, 0);
+    const uint8_t* vp = paged_block(c, page, h, 1);
+    auto scaled = [](uint32_t h2, float f) -> uint32_t {  // the values, rounded to fp16 once
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h2));
+      const __half2 r = __floats2half2_rn(x.x * f, x.y * f);
+      return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    const int g0 = t0 >> 4, g1 = (t1 + 15) >> 4;
+    for (int i = tid; i < (g1 - g0) * D; i += kPagedAppendThreads) {
+      const int g = g0 + i / D, u = i % D;
+      const int ln = u & 31, gq = ln >> 2, q4 = ln & 3;
+      const uint4 xk = *reinterpret_cast<const uint4*>(kp + g * 16 * D + u * 16);
+      const uint4 xv = *reinterpret_cast<const uint4*>(vp + g * 16 * D + u * 16);
+      const uint32_t* wk = reinterpret_cast<const uint32_t*>(&xk);
+      const uint32_t* wv = reinterpret_cast<const uint32_t*>(&xv);
+      const int half = u / 32 / (D / 64), piece = u / 32 % (D / 64);
+      uint32_t o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t lo, hi;
+        codes_to_h2<TIER>(wk[e], lo, hi);
+        o[2 * e] = scaled(lo, sc.x);
+        o[2 * e + 1] = scaled(hi, sc.x);
+      }
+      uint4* kd = reinterpret_cast<uint4*>(sk + (16 * g + 8 * half + gq) * LD + q4 * (D / 4) + piece * 16);
+      kd[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      kd[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      __half* dst = sv + (16 * g + 2 * q4) * LD + gq * (D / 8) + 4 * (u >> 5);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // mb = e >> 1, th = e & 1: (t, j0) (t + 1, j0) (t, j1) (t + 1, j1)
+        uint32_t lo, hi;
+        codes_to_h2<TIER>(wv[e], lo, hi);
+        lo = scaled(lo, sc.y);
+        hi = scaled(hi, sc.y);
+        __half* x = dst + (e & 1) * 8 * LD + (e >> 1) * 2;
+        *reinterpret_cast<uint32_t*>(x) = __byte_perm(lo, hi, 0x5410);
+        *reinterpret_cast<uint32_t*>(x + LD) = __byte_perm(lo, hi, 0x7632);
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < (t1 - t0) * VPR; i += kPagedAppendThreads) {
+    const int t = t0 + i / VPR, d0 = (i % VPR) * 8;
+    const int64_t row = s.row0 + p0 + t - s.start;
+    *reinterpret_cast<uint4*>(k_out + row * ldk + h * D + d0) = *reinterpret_cast<const uint4*>(sk + t * LD + d0);
+    *reinterpret_cast<uint4*>(v_out + row * ldv + h * D + d0) = *reinterpret_cast<const uint4*>(sv + t * LD + d0);
+  }
+}
+
+// ----------------------------------------------------------------------------------
+// the step's work, cut into even ranges
+// ----------------------------------------------------------------------------------
+// A unit is (sequence, KV head, part of its query heads, TQ of its new tokens) against the keys
+// that the last of those tokens sees; its cost is that many keys plus kUnitCost.  All units in
+// a line, ordered by sequence, then head, then token, cost W together; CTA i of n takes the
+// costs [i W / n, (i + 1) W / n): whole units, and parts of at most two, whose partial results
+// (m, l, t, O) the last CTA of the unit to arrive joins in the order of the keys.
+constexpr int64_t kUnitCost = 64;
+
+struct PagedPlan {
+  int G, Gc, hgroups, TQ;  // query heads per KV head, per unit; units per KV head; tokens per unit
+};
+struct PagedSeqCost {
+  int64_t chunks, chain;  // units per (KV head, head part), their cost
+};
+// cost of the first c of a sequence's units (c <= chunks)
+__device__ __forceinline__ int64_t paged_chain(const PagedSeq& s, int TQ, int64_t c) {
+  const int64_t whole = s.n / TQ;  // units with TQ tokens
+  const int64_t w = c < whole ? c : whole;
+  int64_t x = w * (s.start + kUnitCost) + TQ * (w * (w + 1) / 2);
+  if (c > whole) x += s.start + s.n + kUnitCost;
+  return x;
+}
+__device__ __forceinline__ PagedSeqCost paged_cost(const PagedSeq& s, int TQ) {
+  PagedSeqCost r;
+  r.chunks = s.ok ? (s.n + TQ - 1) / TQ : 0;
+  r.chain = paged_chain(s, TQ, r.chunks);
+  if (!s.ok) r.chain = 0;
+  return r;
+}
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+// by one warp: the whole step's cost
+__device__ __forceinline__ int64_t paged_total(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, int lane) {
+  int64_t sum = 0;
+  for (int64_t b = lane; b < st.batch; b += 32) {
+    const PagedSeq s = paged_seq(c, st, b);
+    if (!s.ok) atomicOr(&g_paged_error, kErrPage);
+    sum += paged_cost(s, pl.TQ).chain;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * c.kv_heads * pl.hgroups;
+}
+// by one warp: the sequence at cost x (x < total) and x's distance from its first unit
+__device__ __forceinline__ void paged_locate(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, int64_t x,
+                                             int lane, int64_t& b_out, int64_t& rem) {
+  int64_t before = 0;
+  for (int64_t b0 = 0; b0 < st.batch; b0 += 32) {
+    const int64_t b = b0 + lane;
+    int64_t cost = 0;
+    if (b < st.batch) cost = paged_cost(paged_seq(c, st, b), pl.TQ).chain * c.kv_heads * pl.hgroups;
+    const int64_t incl = warp_scan(cost, lane);
+    const unsigned m = __ballot_sync(0xffffffffu, before + incl > x);
+    if (m) {
+      const int k = __ffs(m) - 1;
+      b_out = b0 + k;
+      rem = x - (before + __shfl_sync(0xffffffffu, incl - cost, k));
+      return;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  b_out = st.batch;  // not reached while x < total
+  rem = 0;
+}
+// CTA that holds cost x when W is dealt to n
+__device__ __forceinline__ int64_t paged_owner(int64_t x, int64_t W, int64_t n) { return ((x + 1) * n + W - 1) / W - 1; }
+
+// ----------------------------------------------------------------------------------
+// attention of few rows
+// ----------------------------------------------------------------------------------
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of fp16, one row of pairs per four lanes, transposed over the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// log2(vs / vref) of a page's V scale: what the exponent of its probabilities is raised by, so
+// that O sums p times codes in units of vref and no code is rounded to take its scale.  Kept
+// within +-60 (a page of zeros has scale 0, and adds zeros whatever the factor); a scale that
+// is not finite gives NaN, and so do the rows that see it.
+__device__ __forceinline__ float v_shift(float vs, float log2_vref) {
+  const float x = fminf(fmaxf(__log2f(vs) - log2_vref, -60.f), 60.f);
+  return vs < __builtin_huge_valf() ? x : __builtin_nanf("");
+}
+
+constexpr int kFewWarps = 4;
+constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kFewTile = 16 * kFewWarps;  // keys per turn of the CTA
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// NB blocks of eight rows (rows = query heads of the unit x its tokens) per unit.  Warp w takes
+// every kFewWarps-th group of 16 keys.  Scores S^T = K Q^T (keys are the MMA's rows, so that
+// eight query rows fill its columns), each lane holding rows 2 q4, 2 q4 + 1 of keys gq, gq + 8;
+// the online softmax per row with a reference that moves only when a score outgrows it by
+// 2^8; P^T, transposed in registers, as the B operand of O^T += V^T P^T, whose columns are the
+// same two rows in every lane.  The next group's codes are loaded before this one is used.
+template <int D, int TIER, int NB>
+struct FewRows {
+  static constexpr int KB = D / 16;
+  static constexpr int R = 8 * NB;
+  uint32_t q[NB][2 * KB];
+  float o[NB][KB][4];
+  float m[NB][2], l[NB][2], t[NB][2];
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < KB; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      m[n][0] = m[n][1] = kNegInf;
+      l[n][0] = l[n][1] = t[n][0] = t[n][1] = 0.f;
+    }
+  }
+  // s: scores of 16 keys from key0; f the factor to base-2 logits, lv / inv the V shift and
+  // 2^-lv; lim: keys that rows 2 q4 (+ 1) of each block see; pb: P^T's B operand
+  __device__ __forceinline__ void softmax(float (&s)[NB][4], float f, float lv, float inv, int64_t key0, bool edge,
+                                          const int64_t (&lim)[NB][2], int gq, uint32_t (&pb)[NB][2]) {
+    bool grow = false;
+    float y[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[n][i] = fmaf(s[n][i], f, lv);
+        if (edge && key0 + gq + (i >> 1) * 8 >= lim[n][i & 1]) y[n][i] = kNegInf;
+      }
+      grow = grow || fmaxf(y[n][0], y[n][2]) > m[n][0] + 8.f || fmaxf(y[n][1], y[n][3]) > m[n][1] + 8.f;
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = fmaxf(y[n][j], y[n][2 + j]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          if (mx > m[n][j]) {
+            const float old = m[n][j];
+            if (old != kNegInf) {
+              const float a = ex2_approx(old - mx);
+              t[n][j] = a * (t[n][j] + l[n][j] * (old - mx));
+              l[n][j] *= a;
+#pragma unroll
+              for (int i = 0; i < KB; ++i) {
+                o[n][i][j] *= a;
+                o[n][i][2 + j] *= a;
+              }
+            }
+            m[n][j] = mx;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float p[4], d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        d[i] = y[n][i] - m[n][i & 1];
+        p[i] = ex2_approx(d[i]);
+        if (edge && y[n][i] == kNegInf) p[i] = d[i] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float sum = p[j] + p[2 + j];
+        l[n][j] = fmaf(inv, sum, l[n][j]);
+        t[n][j] = fmaf(inv, fmaf(-lv, sum, fmaf(p[j], d[j], p[2 + j] * d[2 + j])), t[n][j]);
+      }
+      pb[n][0] = transpose8(pack2(p[0], p[1]));
+      pb[n][1] = transpose8(pack2(p[2], p[3]));
+    }
+  }
+  // 16 keys held in 8 bits
+  __device__ __forceinline__ void codes(const uint4 (&kq)[D / 32], const uint4 (&vq)[D / 32], float f, float lv, float inv,
+                                        int64_t key0, bool edge, const int64_t (&lim)[NB][2], int gq) {
+    float s[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(kq);  // [half][KB] words
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      uint32_t a[4];
+      codes_to_h2<TIER>(kw[kb], a[0], a[2]);
+      codes_to_h2<TIER>(kw[KB + kb], a[1], a[3]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma_16816(s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
+    }
+    uint32_t pb[NB][2];
+    softmax(s, f, lv, inv, key0, edge, lim, gq, pb);
+    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vq);  // [mb][th] words
+#pragma unroll
+    for (int mb = 0; mb < KB; ++mb) {
+      uint32_t a[4];
+      codes_to_h2<TIER>(vw[2 * mb], a[0], a[1]);
+      codes_to_h2<TIER>(vw[2 * mb + 1], a[2], a[3]);
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma_16816(o[n][mb], a, pb[n][0], pb[n][1]);
+    }
+  }
+  // 16 keys held in fp16 (kp / vp: this lane's first unit); tokens from `length` on are not there
+  __device__ __forceinline__ void wide(const uint4* kp, const uint4* vp, float f, float lv, float inv, int64_t key0, bool edge,
+                                       int64_t length, const int64_t (&lim)[NB][2], int gq, int q4) {
+    uint4 ku[D / 16], vu[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) ku[i] = kp[i * 32];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) vu[i] = vp[i * 32];
+    float s[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    const uint32_t* kw = reinterpret_cast<const uint32_t*>(ku);  // [half][KB][2] words
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const uint32_t a[4] = {kw[2 * kb], kw[2 * KB + 2 * kb], kw[2 * kb + 1], kw[2 * KB + 2 * kb + 1]};
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma_16816(s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
+    }
+    uint32_t pb[NB][2];
+    softmax(s, f, lv, inv, key0, edge, lim, gq, pb);
+    uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+    if (key0 + 16 > length) {  // what lies past the sequence's tokens is no number to multiply by
+#pragma unroll
+      for (int th = 0; th < 2; ++th) {
+        const int64_t t0 = key0 + 2 * q4 + 8 * th;
+        keep[th] = (t0 < length ? 0xffffu : 0u) | (t0 + 1 < length ? 0xffff0000u : 0u);
+      }
+    }
+    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vu);
+#pragma unroll
+    for (int mb = 0; mb < KB; ++mb) {
+      const uint32_t a[4] = {vw[4 * mb] & keep[0], vw[4 * mb + 1] & keep[0], vw[4 * mb + 2] & keep[1],
+                             vw[4 * mb + 3] & keep[1]};
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma_16816(o[n][mb], a, pb[n][0], pb[n][1]);
+    }
+  }
+};
+
+template <int D, int TIER, int NB>
+__global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
+    paged_attention_kernel(const PagedArgs c, const PagedStepArgs st, const PagedPlan pl, const PagedRows q, int heads,
+                           float scale, __half* __restrict__ out, int64_t ldo, float* __restrict__ H,
+                           uint32_t* __restrict__ tickets, float* __restrict__ part, int64_t min_cost) {
+  constexpr int R = 8 * NB, KB = D / 16, REC = D + 4;  // record of a row: m, l, t, -, O
+  __shared__ float s_o[kFewWarps][R][D + 4];
+  __shared__ float s_st[kFewWarps][R][3];
+  __shared__ int64_t s_loc[3];
+  __shared__ uint32_t s_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, q4 = lane & 3;
+  griddep_wait();
+  if (warp == 0) {
+    const int64_t W = paged_total(c, st, pl, lane);
+    int64_t n = (W + min_cost - 1) / min_cost;
+    n = n < gridDim.x ? n : gridDim.x;
+    int64_t b = 0, rem = 0;
+    if (blockIdx.x < n) paged_locate(c, st, pl, blockIdx.x * W / n, lane, b, rem);
+    if (lane == 0) {
+      s_loc[0] = W;
+      s_loc[1] = b;
+      s_loc[2] = rem;
+    }
+  }
+  __syncthreads();
+  const int64_t W = s_loc[0];
+  int64_t ncta = (W + min_cost - 1) / min_cost;
+  ncta = ncta < gridDim.x ? ncta : gridDim.x;
+  if (blockIdx.x >= ncta) return;
+  int64_t b = s_loc[1], rem = s_loc[2];
+  int64_t left = (blockIdx.x + 1) * W / ncta - blockIdx.x * W / ncta;  // cost this CTA still has to do
+  const int64_t x0 = blockIdx.x * W / ncta;
+  int64_t done = 0;
+  const float to2 = scale * 1.4426950408889634f;
+
+  FewRows<D, TIER, NB> w;
+  while (left > 0) {
+    const PagedSeq s = paged_seq(c, st, b);
+    const PagedSeqCost sc = paged_cost(s, pl.TQ);
+    const int64_t chains = c.kv_heads * pl.hgroups;
+    if (rem >= sc.chain * chains) {  // on to the next sequence
+      rem -= sc.chain * chains;
+      ++b;
+      if (b >= st.batch) break;
+      continue;
+    }
+    const int64_t ch = rem / sc.chain;
+    int64_t at = rem - ch * sc.chain;  // cost from the chain's start
+    // the unit: the last c0 with chain(c0) <= at
+    int64_t lo = 0, hi = sc.chunks;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (paged_chain(s, pl.TQ, mid) <= at) lo = mid;
+      else hi = mid;
+    }
+    const int64_t unit0 = paged_chain(s, pl.TQ, lo), unit1 = paged_chain(s, pl.TQ, lo + 1);
+    const int64_t h = ch / pl.hgroups;
+    const int hg = static_cast<int>(ch % pl.hgroups);
+    const int64_t tok0 = lo * pl.TQ;
+    const int ntok = static_cast<int>(s.n - tok0 < pl.TQ ? s.n - tok0 : pl.TQ);
+    const int64_t reach = s.start + tok0 + ntok;  // keys that the unit's last token sees
+    const int64_t from = at - unit0, upto = unit1 - unit0 < from + left ? unit1 - unit0 : from + left;
+    const bool whole = from == 0 && upto == unit1 - unit0;
+    auto tile_of = [&](int64_t x) { return x <= kUnitCost ? int64_t(0) : (x - kUnitCost + kFewTile - 1) / kFewTile; };
+    const int64_t g0 = tile_of(from) * kFewWarps;
+    const int64_t groups = (reach + 15) / 16;
+    int64_t g1 = tile_of(upto) * kFewWarps;
+    g1 = g1 < groups ? g1 : groups;
+
+    // rows of the unit: row r = token r / Gc, query head h G + hg Gc + r % Gc
+    auto row_token = [&](int r) { return r / pl.Gc; };
+    auto row_ok = [&](int r) { return r < pl.Gc * pl.TQ && r / pl.Gc < ntok && hg * pl.Gc + r % pl.Gc < pl.G; };
+    int64_t lim[NB][2];
+    w.clear();
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int r = 8 * n + gq;
+      const bool ok = row_ok(r);
+      const int64_t row = s.row0 + tok0 + (ok ? row_token(r) : 0);
+      const int head = static_cast<int>(h) * pl.G + hg * pl.Gc + (ok ? r % pl.Gc : 0);
+      const uint4* src = reinterpret_cast<const uint4*>(q.p + row * q.ld + head * D + q4 * (D / 4));
+#pragma unroll
+      for (int i = 0; i < KB / 2; ++i) {
+        const uint4 x = ok ? src[i] : make_uint4(0, 0, 0, 0);
+        w.q[n][4 * i] = x.x;
+        w.q[n][4 * i + 1] = x.y;
+        w.q[n][4 * i + 2] = x.z;
+        w.q[n][4 * i + 3] = x.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = row_token(8 * n + 2 * q4 + j);
+        lim[n][j] = s.start + tok0 + (t < ntok ? t : ntok - 1) + 1;
+      }
+    }
+    const int64_t sure = s.start + tok0 + 1;  // keys that every row sees
+    const int pg = c.page_shift - 4;          // groups per page, log2
+    const int64_t full = TIER == kFP16 ? c.max_pages : s.length >> c.page_shift;  // blocks in pages
+    const int32_t* table = c.table + s.seq * c.max_pages;
+    auto page_of = [&](int64_t g) -> int {
+      const int64_t blk = g >> pg;
+      if (g >= g1 || blk >= full) return -1;
+      const int p = table[blk];
+      return p >= 0 && p < c.num_pages ? p : -1;
+    };
+    float vref = 1.f;
+    if (TIER != kFP16 && full > 0) {
+      const int p = paged_page(c, s.seq, 0);
+      const float x = p >= 0 ? c.scale[(static_cast<int64_t>(p) * c.kv_heads + h) * 2 + 1] : 1.f;
+      vref = x > 0.f && x < __builtin_huge_valf() ? x : 1.f;
+    }
+    const float log2_vref = __log2f(vref);
+    int64_t g = g0 + warp;
+    if constexpr (TIER != kFP16) {
+      const int64_t gfull = (full << pg) < g1 ? full << pg : g1;  // groups held in 8 bits
+      const int64_t bytes = c.page_size * D;
+      uint4 kq[D / 32], vq[D / 32];
+      float2 sc2 = make_float2(0.f, 0.f);
+      int page = page_of(g), next = page_of(g + kFewWarps);
+      auto load = [&](int64_t gg, int p, uint4 (&ku)[D / 32], uint4 (&vu)[D / 32], float2& f2) {
+        if (p < 0) return;
+        const uint8_t* kp = c.pages + (static_cast<int64_t>(p) * c.kv_heads + h) * 2 * bytes +
+                            (gg & ((1 << pg) - 1)) * 16 * D + lane * 16;
+        const uint8_t* vp = kp + bytes;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) ku[i] = __ldg(reinterpret_cast<const uint4*>(kp + i * 512));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) vu[i] = __ldg(reinterpret_cast<const uint4*>(vp + i * 512));
+        f2 = __ldg(reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + h) * 2));
+      };
+      if (g < gfull) load(g, page, kq, vq, sc2);
+      for (; g < gfull; g += kFewWarps) {
+        uint4 kn[D / 32], vn[D / 32];
+        float2 sn = make_float2(0.f, 0.f);
+        const int after = page_of(g + 2 * kFewWarps);
+        if (g + kFewWarps < gfull) load(g + kFewWarps, next, kn, vn, sn);
+        if (page >= 0) {
+          const float lv = v_shift(sc2.y, log2_vref);
+          w.codes(kq, vq, to2 * sc2.x, lv, ex2_approx(-lv), g * 16, g * 16 + 16 > sure, lim, gq);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          kq[i] = kn[i];
+          vq[i] = vn[i];
+        }
+        sc2 = sn;
+        page = next;
+        next = after;
+      }
+      if (g < g1) {  // the open block
+        const float lv = v_shift(1.f, log2_vref), inv = ex2_approx(-lv);
+        const uint4* ko = reinterpret_cast<const uint4*>(paged_open(c, s.seq, full, h, 0));
+        const uint4* vo = reinterpret_cast<const uint4*>(paged_open(c, s.seq, full, h, 1));
+        for (; g < g1; g += kFewWarps) {
+          const int64_t off = (g - (full << pg)) * 2 * D + lane;
+          w.wide(ko + off, vo + off, to2, lv, inv, g * 16, g * 16 + 16 > sure, s.length, lim, gq, q4);
+        }
+      }
+    } else {
+      for (; g < g1; g += kFewWarps) {
+        const int page = page_of(g);
+        if (page < 0) continue;
+        const uint4* kp = reinterpret_cast<const uint4*>(paged_block(c, page, h, 0)) + (g & ((1 << pg) - 1)) * 2 * D + lane;
+        const uint4* vp = reinterpret_cast<const uint4*>(paged_block(c, page, h, 1)) + (g & ((1 << pg) - 1)) * 2 * D + lane;
+        w.wide(kp, vp, to2, 0.f, 1.f, g * 16, g * 16 + 16 > sure, s.length, lim, gq, q4);
+      }
+    }
+
+    // the warps' rows together
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float l = w.l[n][j], t = w.t[n][j];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          l += __shfl_xor_sync(0xffffffffu, l, o);
+          t += __shfl_xor_sync(0xffffffffu, t, o);
+        }
+        const int r = 8 * n + 2 * q4 + j;
+        if (gq == 0) {
+          s_st[warp][r][0] = w.m[n][j];
+          s_st[warp][r][1] = l;
+          s_st[warp][r][2] = t;
+        }
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          s_o[warp][r][gq * (D / 8) + 2 * i] = w.o[n][i][j];
+          s_o[warp][r][gq * (D / 8) + 2 * i + 1] = w.o[n][i][2 + j];
+        }
+      }
+    }
+    __syncthreads();
+    // one row of results: (m, l, t) and the columns this thread sums
+    auto finish = [&](int r, int col, float L, float T, float O) {
+      const int64_t row = s.row0 + tok0 + row_token(r);
+      const int head = static_cast<int>(h) * pl.G + hg * pl.Gc + r % pl.Gc;
+      const bool some = L != 0.f;  // a row that sees no key: zeros
+      out[row * ldo + head * D + col] = __float2half_rn(some ? O * vref / L : 0.f);
+      if (col == 0 && H != nullptr)
+        H[row * heads + head] = some ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
+    };
+    const int64_t first = paged_owner(x0 + done - from, W, ncta);  // CTAs that share the unit: first .. last
+    const int64_t last = paged_owner(x0 + done - from + (unit1 - unit0) - 1, W, ncta);
+    for (int i = tid; i < R * D; i += kFewThreads) {
+      const int r = i / D, col = i % D;
+      if (!row_ok(r)) continue;
+      float M = kNegInf, L = 0.f, T = 0.f, O = 0.f;
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) M = fmaxf(M, s_st[k][r][0]);
+#pragma unroll
+      for (int k = 0; k < kFewWarps; ++k) {
+        const float mk = s_st[k][r][0], lk = s_st[k][r][1];
+        if (mk == kNegInf && lk == 0.f) continue;  // saw no key (NaN sums go on)
+        const float a = mk == kNegInf ? 1.f : ex2_approx(mk - M);
+        L += a * lk;
+        T += a * (s_st[k][r][2] + (mk == kNegInf ? 0.f : lk * (mk - M)));
+        O += a * s_o[k][r][col];
+      }
+      if (whole) {
+        finish(r, col, L, T, O);
+      } else {
+        float* rec = part + ((2 * blockIdx.x + (from == 0 ? 1 : 0)) * R + r) * REC;
+        rec[4 + col] = O;
+        if (col == 0) *reinterpret_cast<float4*>(rec) = make_float4(M, L, T, 0.f);
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        s_last = atomicAdd(&tickets[first], 1u) == static_cast<uint32_t>(last - first);
+        if (s_last) tickets[first] = 0;  // left as it was found
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        for (int i = tid; i < R * D; i += kFewThreads) {
+          const int r = i / D, col = i % D;
+          if (!row_ok(r)) continue;
+          float M = kNegInf, L = 0.f, T = 0.f, O = 0.f;
+          for (int64_t k = first; k <= last; ++k) {
+            const float* rec = part + ((2 * k + (k == first ? 1 : 0)) * R + r) * REC;
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec));
+            if (x.x == kNegInf && x.y == 0.f) continue;
+            const float o = __ldcg(rec + 4 + col);
+            const float mn = fmaxf(M, x.x);
+            const float a = M == kNegInf ? (mn == kNegInf ? 1.f : 0.f) : ex2_approx(M - mn);
+            const float e = x.x == kNegInf ? 1.f : ex2_approx(x.x - mn);
+            T = (M == kNegInf ? 0.f : a * (T + L * (M - mn))) + e * (x.z + (x.x == kNegInf ? 0.f : x.y * (x.x - mn)));
+            L = a * L + e * x.y;
+            O = a * O + e * o;
+            M = mn;
+          }
+          finish(r, col, L, T, O);
+        }
+      }
+    }
+    __syncthreads();  // the shared rows are free again
+    rem += upto - from;
+    done += upto - from;
+    left -= upto - from;
+  }
+}
+
+}  // namespace ee

@@ -1,0 +1,243 @@
+"""Paged KV cache for serving: sequences of different lengths in one step, prefill in chunks,
+pages that are handed out and given back (include/ee_b200.h, ``ee_paged_*``).
+
+The cache keeps keys and values in one precision tier: INT8 or FP8 codes with one scale for
+each page and KV head, or FP16.  A page's tokens are quantised when the page is full; until
+then they stay in fp16.  ``PagedKVCache.attention`` returns, like the other attention entry
+points, every query row's entropy: the router input of the token's MLP.
+
+    cache = PagedKVCache(max_seqs=64, num_pages=8192, page_size=64, kv_heads=8, head_dim=128)
+    step = cache.step([3, 5], counts=[700, 1])       # a prompt for one sequence, a token for another
+    q = cache.append(k, v, step, cos=cos, sin=sin, q=q)
+    out, H = cache.attention(q, step)
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Dict, List, Optional, Sequence
+
+import torch
+
+from . import _lib
+from ._lib import call
+from .dispatch import PrecisionTier
+from .kernels import _check_cuda, _require, _stream
+
+
+class _PagedCacheC(ctypes.Structure):
+    _fields_ = [("num_pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("max_seqs", ctypes.c_int64), ("max_pages", ctypes.c_int64),
+                ("tier", ctypes.c_int32), ("pages", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("open", ctypes.c_void_p), ("table", ctypes.c_void_p)]
+
+
+class _PagedStepC(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("rows", ctypes.c_int64), ("max_new", ctypes.c_int64),
+                ("seq", ctypes.c_void_p), ("start", ctypes.c_void_p), ("length", ctypes.c_void_p),
+                ("cu", ctypes.c_void_p)]
+
+
+class PagedStep:
+    """The sequences of one call: sequence ``seqs[b]`` has the rows ``cu[b] .. cu[b + 1] - 1``,
+    its tokens at positions ``starts[b] ..`` of ``lengths[b]``.  One host-to-device copy."""
+
+    def __init__(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int], lengths: Sequence[int],
+                 device):
+        n = len(seqs)
+        cu = [0]
+        for c in counts:
+            cu.append(cu[-1] + c)
+        self.seqs, self.starts, self.counts, self.lengths = list(seqs), list(starts), list(counts), list(lengths)
+        self.rows = cu[-1]
+        self.arrays = torch.tensor(self.seqs + self.starts + self.lengths + cu, dtype=torch.int32, device=device)
+        base = self.arrays.data_ptr()
+        self.c = _PagedStepC(n, self.rows, max(counts, default=0), base, base + 4 * n, base + 8 * n, base + 12 * n)
+
+
+class PagedKVCache:
+    """Room for ``max_seqs`` sequences of up to ``max_pages`` pages each (default: the whole
+    pool), ``num_pages`` pages of ``page_size`` tokens (16, 32, 64 or 128) between them, with
+    ``kv_heads`` heads of ``head_dim`` (64 or 128), in precision ``tier``."""
+
+    def __init__(self, max_seqs: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
+                 max_pages: Optional[int] = None, tier: PrecisionTier = PrecisionTier.INT8, device="cuda"):
+        self.max_seqs, self.num_pages, self.page_size = int(max_seqs), int(num_pages), int(page_size)
+        self.kv_heads, self.head_dim, self.tier = int(kv_heads), int(head_dim), PrecisionTier(int(tier))
+        self.max_pages = self.num_pages if max_pages is None else int(max_pages)
+        shape = (self.num_pages, self.kv_heads, self.head_dim, self.page_size, self.max_seqs, self.max_pages,
+                 int(self.tier))
+        lib = _lib.load()
+        nbytes = lib.ee_paged_cache_bytes(*shape)
+        _require(nbytes > 0, "unsupported paged-cache shape (head_dim 64 or 128, pages of 16, 32, 64 or 128 tokens)")
+        self.device = torch.device(device)
+        self.memory = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self.device = self.memory.device
+        self.c = _PagedCacheC()
+        with torch.cuda.device(self.device):
+            call("ee_paged_cache_init", ctypes.byref(self.c), self.memory.data_ptr(), nbytes, *shape, _stream())
+        off = self.c.table - self.memory.data_ptr()
+        self.table = self.memory[off:off + 4 * self.max_seqs * self.max_pages].view(torch.int32).view(self.max_seqs,
+                                                                                                   self.max_pages)
+        self.lengths: List[int] = [0] * self.max_seqs  # tokens of each sequence, as appended
+        self._wide: List[int] = [0] * self.max_seqs  # first block whose fp16 rows are at hand (8-bit tiers)
+        self._pages: List[List[int]] = [[] for _ in range(self.max_seqs)]
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._changed: Dict[int, int] = {}  # table entries not on the device yet
+        self._ws: Dict[int, torch.Tensor] = {}  # workspace of each stream
+
+    # ------------------------------------------------------------------ pages
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _seq(self, seq: int) -> int:
+        _require(0 <= int(seq) < self.max_seqs, f"sequence {seq} is outside 0 .. {self.max_seqs - 1}")
+        return int(seq)
+
+    def reserve(self, seq: int, tokens: int) -> None:
+        """Hands out pages until sequence ``seq`` has room for ``tokens`` tokens."""
+        seq = self._seq(seq)
+        have = self._pages[seq]
+        need = -(-int(tokens) // self.page_size)
+        _require(need <= self.max_pages, f"{tokens} tokens are more than {self.max_pages} pages hold")
+        _require(need - len(have) <= len(self._free),
+                 f"the cache is full: {need - len(have)} pages wanted, {len(self._free)} free")
+        while len(have) < need:
+            page = self._free.pop()
+            self._changed[seq * self.max_pages + len(have)] = page
+            have.append(page)
+
+    def release(self, seq: int) -> None:
+        """Gives a sequence's pages back; its slot starts anew."""
+        seq = self._seq(seq)
+        for i in range(len(self._pages[seq])):
+            self._changed[seq * self.max_pages + i] = -1
+        self._free.extend(reversed(self._pages[seq]))
+        self._pages[seq] = []
+        self.lengths[seq] = self._wide[seq] = 0
+
+    def truncate(self, seq: int, tokens: int) -> None:
+        """Takes a sequence's last tokens back (drafted tokens that were not accepted).  In the
+        8-bit tiers the new end is at most ``page_size`` tokens back (the fp16 rows of the open
+        block and the one before it are still there), or a page's end."""
+        seq, tokens, n = self._seq(seq), int(tokens), self.lengths[seq]
+        _require(0 <= tokens <= n, f"sequence {seq} has {n} tokens")
+        first = self._wide[seq] * self.page_size
+        _require(self.tier == PrecisionTier.FP16 or tokens >= first or tokens % self.page_size == 0,
+                 f"sequence {seq} can be cut to {first} or more tokens, or to whole pages")
+        self.lengths[seq] = tokens
+        self._wide[seq] = min(self._wide[seq], tokens // self.page_size)
+
+    def _upload(self) -> None:
+        if self._changed:
+            at = torch.tensor([list(self._changed), list(self._changed.values())], dtype=torch.int64,
+                              device=self.device)
+            self.table.view(-1)[at[0]] = at[1].to(torch.int32)
+            self._changed = {}
+
+    # ------------------------------------------------------------------ steps
+    def step(self, seqs: Sequence[int], starts: Optional[Sequence[int]] = None, counts: Optional[Sequence[int]] = None
+             ) -> PagedStep:
+        """``counts[b]`` new tokens (default one) for each sequence of ``seqs``, from its end on
+        or from position ``starts[b]``; hands out the pages they need."""
+        seqs = [self._seq(s) for s in seqs]
+        _require(len(set(seqs)) == len(seqs), "a sequence occurs once in a step")
+        starts = [self.lengths[s] for s in seqs] if starts is None else [int(x) for x in starts]
+        counts = [1] * len(seqs) if counts is None else [int(x) for x in counts]
+        _require(len(starts) == len(seqs) and len(counts) == len(seqs), "one start and one count per sequence")
+        _require(all(x >= 0 for x in starts) and all(x >= 0 for x in counts), "starts and counts must be >= 0")
+        ends = [a + n for a, n in zip(starts, counts)]
+        for s, e in zip(seqs, ends):
+            self.reserve(s, e)
+        self._upload()
+        return PagedStep(seqs, starts, counts, ends, self.device)
+
+    def span(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int]) -> PagedStep:
+        """Tokens ``starts[b] ..`` of sequences as they are cached, for ``read``."""
+        seqs = [self._seq(s) for s in seqs]
+        starts, counts = [int(x) for x in starts], [int(x) for x in counts]
+        _require(len(starts) == len(seqs) and len(counts) == len(seqs), "one start and one count per sequence")
+        _require(all(a >= 0 and n >= 0 and a + n <= self.lengths[s] for s, a, n in zip(seqs, starts, counts)),
+                 "a span lies inside its sequence")
+        self._upload()
+        return PagedStep(seqs, starts, counts, [self.lengths[s] for s in seqs], self.device)
+
+    def _rows(self, x: torch.Tensor, name: str, step: PagedStep, width: int) -> torch.Tensor:
+        _check_cuda(x, name)
+        _require(x.dtype == torch.float16 and x.dim() == 2 and x.shape[0] == step.rows and x.shape[1] == width,
+                 f"{name} must be fp16 [{step.rows}, {width}]")
+        _require(x.device == self.device and step.arrays.device == self.device, f"{name} must be on {self.device}")
+        _require(x.stride(1) == 1, f"{name} needs unit column stride")
+        return x
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep, cos: Optional[torch.Tensor] = None,
+               sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+               out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """Appends the step's rows k, v (fp16 [rows, kv_heads * head_dim]).  With ``cos`` / ``sin``
+        (fp16 [rows, head_dim]) k is rotated on the way in, and ``q`` (fp16 [rows, heads *
+        head_dim]) with it: returned (in ``out`` when given, which may be ``q``)."""
+        width = self.kv_heads * self.head_dim
+        self._rows(k, "k", step, width)
+        self._rows(v, "v", step, width)
+        _require((cos is None) == (sin is None), "cos and sin go together")
+        if cos is not None:
+            self._rows(cos, "cos", step, self.head_dim)
+            self._rows(sin, "sin", step, self.head_dim)
+            _require(cos.stride(0) == sin.stride(0), "cos and sin need one row stride")
+        heads, y = 0, None
+        if q is not None:
+            _require(q.dim() == 2 and q.shape[1] % self.head_dim == 0, "q must be fp16 [rows, heads * head_dim]")
+            heads = q.shape[1] // self.head_dim
+            self._rows(q, "q", step, q.shape[1])
+            y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else self._rows(out, "out", step,
+                                                                                                   q.shape[1])
+        with torch.cuda.device(self.device):
+            call("ee_paged_append", ctypes.byref(self.c), ctypes.byref(step.c), k.data_ptr(), k.stride(0), v.data_ptr(),
+                 v.stride(0), None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
+                 0 if cos is None else cos.stride(0), None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
+                 heads, None if y is None else y.data_ptr(), 0 if y is None else y.stride(0), _stream())
+        for s, a, n in zip(step.seqs, step.starts, step.counts):
+            if n:
+                first, last = a // self.page_size, (a + n - 1) // self.page_size
+                # an append that goes on where the sequence ended keeps the block before, too
+                kept = min(self._wide[s], first) if a == self.lengths[s] else first
+                self._wide[s] = max(kept, last - 1)
+                self.lengths[s] = a + n
+        return y
+
+    def attention(self, q: torch.Tensor, step: PagedStep, scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None):
+        """Causal attention of the step's rows q (fp16 [rows, heads * head_dim], rotated), after
+        their append: (out fp16 [rows, heads * head_dim], H fp32 [rows, heads], the entropy of
+        each softmax row)."""
+        _require(q.dim() == 2 and q.shape[1] % (self.kv_heads * self.head_dim) == 0,
+                 "q must be fp16 [rows, heads * head_dim], heads a multiple of kv_heads")
+        self._rows(q, "q", step, q.shape[1])
+        heads = q.shape[1] // self.head_dim
+        y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else self._rows(out, "out", step,
+                                                                                               q.shape[1])
+        H = torch.empty(step.rows, heads, dtype=torch.float32, device=q.device)
+        with torch.cuda.device(self.device):
+            stream = _stream()
+            ws = self._ws.get(stream)
+            if ws is None:  # zeroed once; the kernel leaves its head zero
+                ws = self._ws[stream] = torch.zeros(_lib.load().ee_paged_workspace_bytes(ctypes.byref(self.c)),
+                                                    dtype=torch.uint8, device=self.device)
+            call("ee_paged_attention", ctypes.byref(self.c), ctypes.byref(step.c), q.data_ptr(), q.stride(0), heads,
+                 float(self.head_dim ** -0.5 if scale is None else scale), y.data_ptr(), y.stride(0), H.data_ptr(),
+                 ws.data_ptr(), ws.numel(), stream)
+        return y, H
+
+    def read(self, span: PagedStep):
+        """(k, v) fp16 [rows, kv_heads * head_dim] of a span: the values the cache stands for."""
+        k = torch.empty(span.rows, self.kv_heads * self.head_dim, dtype=torch.float16, device=self.device)
+        v = torch.empty_like(k)
+        with torch.cuda.device(self.device):
+            call("ee_paged_read", ctypes.byref(self.c), ctypes.byref(span.c), k.data_ptr(), k.stride(0), v.data_ptr(),
+                 v.stride(0), _stream())
+        return k, v
+
+    def bytes_per_token(self) -> float:
+        """Bytes a token of a full page takes (keys and values of every KV head, with scales)."""
+        row = 2 * self.kv_heads * self.head_dim
+        return 2.0 * row if self.tier == PrecisionTier.FP16 else row + 8.0 * self.kv_heads / self.page_size
