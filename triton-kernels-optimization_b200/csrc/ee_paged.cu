@@ -7,6 +7,7 @@
 #include <utility>
 
 #include "ee_paged.cuh"
+#include "ee_paged_chunk.cuh"
 
 namespace ee {
 
@@ -72,31 +73,51 @@ constexpr int few_ctas(int nb) { return nb == 1 ? 3 : 2; }
 template <int D, int TIER, int NB>
 int run_few(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, const PagedRows& q, int heads, float scale,
             __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
-  // no CTA for less than four turns of its warps: shorter parts cost more in joining than
-  // they save
   return launch_pdl(paged_attention_kernel<D, TIER, NB>, dim3(static_cast<unsigned>(sm_count() * few_ctas(NB))),
-                    dim3(kFewThreads), 0, s, c, st, pl, q, heads, scale, out, ldo, H, tickets, part,
-                    int64_t(4 * kFewTile));
+                    dim3(kFewThreads), 0, s, c, st, pl, q, heads, scale, out, ldo, H, tickets, part);
+}
+template <int D, int TIER>
+int run_chunk(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, const PagedRows& q, int heads, float scale,
+              __half* out, int64_t ldo, float* H, float* part, cudaStream_t s) {
+  int e = allow_smem<paged_chunk_kernel<D, TIER>>(ChunkCfg<D>::kSmem);
+  if (e != 0) return e;
+  const unsigned n = static_cast<unsigned>(sm_count());
+  e = launch_pdl(paged_chunk_kernel<D, TIER>, dim3(n), dim3(kChunkThreads), ChunkCfg<D>::kSmem, s, c, st, pl, q, heads,
+                 scale, out, ldo, H, part);
+  if (e != 0) return e;
+  return launch_pdl(paged_join_kernel<D>, dim3(n, 8), dim3(256), 0, s, c, st, pl, heads, out, ldo, H,
+                    static_cast<const float*>(part));
 }
 template <int D, int TIER>
 int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new, float scale,
                   __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
   const int G = heads / static_cast<int>(c.kv_heads);
-  const bool one = G * max_new <= 8;
+  // query rows of one KV head that a unit holds: 8 or 16 (mma.sync, bound by the cache's
+  // bytes), or two tiles of 128 (tcgen05)
+  const int64_t rows = G * max_new;
+  const int R = rows <= 8 ? 8 : (rows <= 16 ? 16 : 128);
   PagedPlan pl;
-  const int R = one ? 8 : 16;
   pl.G = G;
   pl.hgroups = (G + R - 1) / R;
   pl.Gc = (G + pl.hgroups - 1) / pl.hgroups;
   pl.TQ = R / pl.Gc;
-  if (one) return run_few<D, TIER, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
-  return run_few<D, TIER, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  pl.fixed = 64;
+  // no CTA for less than four turns of its warps: shorter parts cost more in joining than
+  // they save
+  pl.min_cost = 4 * kFewTile;
+  if (R == 8) return run_few<D, TIER, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  if (R == 16) return run_few<D, TIER, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  pl.TQ *= 2;
+  pl.fixed = 2 * kChunkTile;
+  pl.min_cost = 4 * kChunkTile;
+  return run_chunk<D, TIER>(c, st, pl, q, heads, scale, out, ldo, H, part, s);
 }
 }  // namespace
 
 size_t paged_head_bytes() { return 4096; }  // a ticket per CTA
 size_t paged_workspace_bytes(int64_t D) {
-  return paged_head_bytes() + size_t(2) * sm_count() * few_ctas(1) * 16 * (D + 4) * sizeof(float);
+  // two parts per CTA: 16 rows of the few-row kernel's CTAs, 256 of the chunk kernel's
+  return paged_head_bytes() + size_t(2) * sm_count() * std::max<size_t>(few_ctas(1) * 16 * (D + 4), 256 * (D + 3)) * sizeof(float);
 }
 
 #define EE_PAGED_DISPATCH(call)                                            \

@@ -503,30 +503,31 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
 // the step's work, cut into even ranges
 // ----------------------------------------------------------------------------------
 // A unit is (sequence, KV head, part of its query heads, TQ of its new tokens) against the keys
-// that the last of those tokens sees; its cost is that many keys plus kUnitCost.  All units in
+// that the last of those tokens sees; its cost is that many keys plus PagedPlan::fixed, what a
+// unit costs whatever its length.  All units in
 // a line, ordered by sequence, then head, then token, cost W together; CTA i of n takes the
 // costs [i W / n, (i + 1) W / n): whole units, and parts of at most two, whose partial results
 // (m, l, t, O) the last CTA of the unit to arrive joins in the order of the keys.
-constexpr int64_t kUnitCost = 64;
-
 struct PagedPlan {
   int G, Gc, hgroups, TQ;  // query heads per KV head, per unit; units per KV head; tokens per unit
+  int fixed;               // a unit's fixed cost, in keys
+  int64_t min_cost;        // no CTA for less
 };
 struct PagedSeqCost {
   int64_t chunks, chain;  // units per (KV head, head part), their cost
 };
 // cost of the first c of a sequence's units (c <= chunks)
-__device__ __forceinline__ int64_t paged_chain(const PagedSeq& s, int TQ, int64_t c) {
-  const int64_t whole = s.n / TQ;  // units with TQ tokens
+__device__ __forceinline__ int64_t paged_chain(const PagedSeq& s, const PagedPlan& pl, int64_t c) {
+  const int64_t whole = s.n / pl.TQ;  // units with TQ tokens
   const int64_t w = c < whole ? c : whole;
-  int64_t x = w * (s.start + kUnitCost) + TQ * (w * (w + 1) / 2);
-  if (c > whole) x += s.start + s.n + kUnitCost;
+  int64_t x = w * (s.start + pl.fixed) + pl.TQ * (w * (w + 1) / 2);
+  if (c > whole) x += s.start + s.n + pl.fixed;
   return x;
 }
-__device__ __forceinline__ PagedSeqCost paged_cost(const PagedSeq& s, int TQ) {
+__device__ __forceinline__ PagedSeqCost paged_cost(const PagedSeq& s, const PagedPlan& pl) {
   PagedSeqCost r;
-  r.chunks = s.ok ? (s.n + TQ - 1) / TQ : 0;
-  r.chain = paged_chain(s, TQ, r.chunks);
+  r.chunks = s.ok ? (s.n + pl.TQ - 1) / pl.TQ : 0;
+  r.chain = paged_chain(s, pl, r.chunks);
   if (!s.ok) r.chain = 0;
   return r;
 }
@@ -544,7 +545,7 @@ __device__ __forceinline__ int64_t paged_total(const PagedArgs& c, const PagedSt
   for (int64_t b = lane; b < st.batch; b += 32) {
     const PagedSeq s = paged_seq(c, st, b);
     if (!s.ok) atomicOr(&g_paged_error, kErrPage);
-    sum += paged_cost(s, pl.TQ).chain;
+    sum += paged_cost(s, pl).chain;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -557,7 +558,7 @@ __device__ __forceinline__ void paged_locate(const PagedArgs& c, const PagedStep
   for (int64_t b0 = 0; b0 < st.batch; b0 += 32) {
     const int64_t b = b0 + lane;
     int64_t cost = 0;
-    if (b < st.batch) cost = paged_cost(paged_seq(c, st, b), pl.TQ).chain * c.kv_heads * pl.hgroups;
+    if (b < st.batch) cost = paged_cost(paged_seq(c, st, b), pl).chain * c.kv_heads * pl.hgroups;
     const int64_t incl = warp_scan(cost, lane);
     const unsigned m = __ballot_sync(0xffffffffu, before + incl > x);
     if (m) {
@@ -573,6 +574,101 @@ __device__ __forceinline__ void paged_locate(const PagedArgs& c, const PagedStep
 }
 // CTA that holds cost x when W is dealt to n
 __device__ __forceinline__ int64_t paged_owner(int64_t x, int64_t W, int64_t n) { return ((x + 1) * n + W - 1) / W - 1; }
+
+// Where a CTA's share of the line stands.  paged_begin: by the whole block (share: three words of
+// shared memory); ncta: CTAs that have a share.
+struct PagedWalk {
+  int64_t W, ncta, x0, b, rem, left, done;
+};
+__device__ __forceinline__ PagedWalk paged_begin(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, int64_t cta,
+                                                 int64_t ctas, int64_t* share) {
+  auto count = [&](int64_t W) {
+    const int64_t n = (W + pl.min_cost - 1) / pl.min_cost;
+    return n < ctas ? n : ctas;
+  };
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    const int64_t W = paged_total(c, st, pl, lane), n = count(W);
+    int64_t b = 0, rem = 0;
+    if (cta < n) paged_locate(c, st, pl, cta * W / n, lane, b, rem);
+    if (lane == 0) {
+      share[0] = W;
+      share[1] = b;
+      share[2] = rem;
+    }
+  }
+  __syncthreads();
+  PagedWalk w;
+  w.W = share[0];
+  w.b = share[1];
+  w.rem = share[2];
+  w.ncta = count(w.W);
+  w.done = 0;
+  w.x0 = w.left = 0;
+  if (cta < w.ncta) {
+    w.x0 = cta * w.W / w.ncta;
+    w.left = (cta + 1) * w.W / w.ncta - w.x0;
+  }
+  return w;
+}
+// The part of the next unit that falls into the share: keys of tiles [tile0, tile1) of TILE.
+struct PagedPart {
+  PagedSeq s;
+  int h, hg, ntok;            // KV head, part of its query heads, tokens of the unit
+  int64_t tok0, reach;        // first token; keys that the last one sees
+  int tile0, tile1;
+  bool first, whole;          // begins the unit; is all of it
+  int64_t cta0, cta1;         // the CTAs that share the unit
+};
+template <int TILE>
+__device__ __forceinline__ bool paged_next(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, PagedWalk& w,
+                                           PagedPart& p) {
+  const int64_t chains = c.kv_heads * pl.hgroups;
+  while (w.left > 0 && w.b < st.batch) {
+    p.s = paged_seq(c, st, w.b);
+    const PagedSeqCost sc = paged_cost(p.s, pl);
+    if (w.rem >= sc.chain * chains) {  // on to the next sequence
+      w.rem -= sc.chain * chains;
+      ++w.b;
+      continue;
+    }
+    const int64_t ch = w.rem / sc.chain;
+    const int64_t at = w.rem - ch * sc.chain;  // cost from the chain's start
+    int64_t lo = 0, hi = sc.chunks;            // the unit: the last with chain(lo) <= at
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (paged_chain(p.s, pl, mid) <= at) lo = mid;
+      else hi = mid;
+    }
+    const int64_t unit0 = paged_chain(p.s, pl, lo), cost = paged_chain(p.s, pl, lo + 1) - unit0;
+    p.h = static_cast<int>(ch / pl.hgroups);
+    p.hg = static_cast<int>(ch % pl.hgroups);
+    p.tok0 = lo * pl.TQ;
+    p.ntok = static_cast<int>(p.s.n - p.tok0 < pl.TQ ? p.s.n - p.tok0 : pl.TQ);
+    p.reach = p.s.start + p.tok0 + p.ntok;
+    const int64_t from = at - unit0, upto = cost < from + w.left ? cost : from + w.left;
+    auto tile = [&](int64_t x) { return x <= pl.fixed ? 0 : static_cast<int>((x - pl.fixed + TILE - 1) / TILE); };
+    p.tile0 = tile(from);
+    p.tile1 = tile(upto);
+    p.first = from == 0;
+    p.whole = p.first && upto == cost;
+    const int64_t x = w.x0 + w.done - from;  // the unit's place in the line
+    p.cta0 = p.whole ? 0 : paged_owner(x, w.W, w.ncta);
+    p.cta1 = p.whole ? 0 : paged_owner(x + cost - 1, w.W, w.ncta);
+    w.rem += upto - from;
+    w.done += upto - from;
+    w.left -= upto - from;
+    return true;
+  }
+  return false;
+}
+// reference of the V scales of a (sequence, KV head): its first page's
+__device__ __forceinline__ float paged_vref(const PagedArgs& c, const PagedSeq& s, int h) {
+  if (c.tier == kFP16 || s.length < c.page_size) return 1.f;
+  const int p = paged_page(c, s.seq, 0);
+  const float x = p >= 0 ? c.scale[(static_cast<int64_t>(p) * c.kv_heads + h) * 2 + 1] : 1.f;
+  return x > 0.f && x < __builtin_huge_valf() ? x : 1.f;
+}
 
 // ----------------------------------------------------------------------------------
 // attention of few rows
@@ -768,69 +864,27 @@ template <int D, int TIER, int NB>
 __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
     paged_attention_kernel(const PagedArgs c, const PagedStepArgs st, const PagedPlan pl, const PagedRows q, int heads,
                            float scale, __half* __restrict__ out, int64_t ldo, float* __restrict__ H,
-                           uint32_t* __restrict__ tickets, float* __restrict__ part, int64_t min_cost) {
+                           uint32_t* __restrict__ tickets, float* __restrict__ part) {
   constexpr int R = 8 * NB, KB = D / 16, REC = D + 4;  // record of a row: m, l, t, -, O
   __shared__ float s_o[kFewWarps][R][D + 4];
   __shared__ float s_st[kFewWarps][R][3];
-  __shared__ int64_t s_loc[3];
+  __shared__ int64_t s_share[3];
   __shared__ uint32_t s_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, q4 = lane & 3;
   griddep_wait();
-  if (warp == 0) {
-    const int64_t W = paged_total(c, st, pl, lane);
-    int64_t n = (W + min_cost - 1) / min_cost;
-    n = n < gridDim.x ? n : gridDim.x;
-    int64_t b = 0, rem = 0;
-    if (blockIdx.x < n) paged_locate(c, st, pl, blockIdx.x * W / n, lane, b, rem);
-    if (lane == 0) {
-      s_loc[0] = W;
-      s_loc[1] = b;
-      s_loc[2] = rem;
-    }
-  }
-  __syncthreads();
-  const int64_t W = s_loc[0];
-  int64_t ncta = (W + min_cost - 1) / min_cost;
-  ncta = ncta < gridDim.x ? ncta : gridDim.x;
-  if (blockIdx.x >= ncta) return;
-  int64_t b = s_loc[1], rem = s_loc[2];
-  int64_t left = (blockIdx.x + 1) * W / ncta - blockIdx.x * W / ncta;  // cost this CTA still has to do
-  const int64_t x0 = blockIdx.x * W / ncta;
-  int64_t done = 0;
+  PagedWalk walk = paged_begin(c, st, pl, blockIdx.x, gridDim.x, s_share);
   const float to2 = scale * 1.4426950408889634f;
 
   FewRows<D, TIER, NB> w;
-  while (left > 0) {
-    const PagedSeq s = paged_seq(c, st, b);
-    const PagedSeqCost sc = paged_cost(s, pl.TQ);
-    const int64_t chains = c.kv_heads * pl.hgroups;
-    if (rem >= sc.chain * chains) {  // on to the next sequence
-      rem -= sc.chain * chains;
-      ++b;
-      if (b >= st.batch) break;
-      continue;
-    }
-    const int64_t ch = rem / sc.chain;
-    int64_t at = rem - ch * sc.chain;  // cost from the chain's start
-    // the unit: the last c0 with chain(c0) <= at
-    int64_t lo = 0, hi = sc.chunks;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (paged_chain(s, pl.TQ, mid) <= at) lo = mid;
-      else hi = mid;
-    }
-    const int64_t unit0 = paged_chain(s, pl.TQ, lo), unit1 = paged_chain(s, pl.TQ, lo + 1);
-    const int64_t h = ch / pl.hgroups;
-    const int hg = static_cast<int>(ch % pl.hgroups);
-    const int64_t tok0 = lo * pl.TQ;
-    const int ntok = static_cast<int>(s.n - tok0 < pl.TQ ? s.n - tok0 : pl.TQ);
-    const int64_t reach = s.start + tok0 + ntok;  // keys that the unit's last token sees
-    const int64_t from = at - unit0, upto = unit1 - unit0 < from + left ? unit1 - unit0 : from + left;
-    const bool whole = from == 0 && upto == unit1 - unit0;
-    auto tile_of = [&](int64_t x) { return x <= kUnitCost ? int64_t(0) : (x - kUnitCost + kFewTile - 1) / kFewTile; };
-    const int64_t g0 = tile_of(from) * kFewWarps;
-    const int64_t groups = (reach + 15) / 16;
-    int64_t g1 = tile_of(upto) * kFewWarps;
+  PagedPart u;
+  while (paged_next<kFewTile>(c, st, pl, walk, u)) {
+    const PagedSeq& s = u.s;
+    const int64_t tok0 = u.tok0, h = u.h;
+    const int ntok = u.ntok, hg = u.hg;
+    const bool whole = u.whole;
+    const int64_t g0 = static_cast<int64_t>(u.tile0) * kFewWarps;
+    const int64_t groups = (u.reach + 15) / 16;
+    int64_t g1 = static_cast<int64_t>(u.tile1) * kFewWarps;
     g1 = g1 < groups ? g1 : groups;
 
     // rows of the unit: row r = token r / Gc, query head h G + hg Gc + r % Gc
@@ -869,12 +923,7 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
       const int p = table[blk];
       return p >= 0 && p < c.num_pages ? p : -1;
     };
-    float vref = 1.f;
-    if (TIER != kFP16 && full > 0) {
-      const int p = paged_page(c, s.seq, 0);
-      const float x = p >= 0 ? c.scale[(static_cast<int64_t>(p) * c.kv_heads + h) * 2 + 1] : 1.f;
-      vref = x > 0.f && x < __builtin_huge_valf() ? x : 1.f;
-    }
+    const float vref = paged_vref(c, s, u.h);
     const float log2_vref = __log2f(vref);
     int64_t g = g0 + warp;
     if constexpr (TIER != kFP16) {
@@ -966,8 +1015,7 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
       if (col == 0 && H != nullptr)
         H[row * heads + head] = some ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
     };
-    const int64_t first = paged_owner(x0 + done - from, W, ncta);  // CTAs that share the unit: first .. last
-    const int64_t last = paged_owner(x0 + done - from + (unit1 - unit0) - 1, W, ncta);
+    const int64_t first = u.cta0, last = u.cta1;
     for (int i = tid; i < R * D; i += kFewThreads) {
       const int r = i / D, col = i % D;
       if (!row_ok(r)) continue;
@@ -986,7 +1034,7 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
       if (whole) {
         finish(r, col, L, T, O);
       } else {
-        float* rec = part + ((2 * blockIdx.x + (from == 0 ? 1 : 0)) * R + r) * REC;
+        float* rec = part + ((2 * blockIdx.x + (u.first ? 1 : 0)) * R + r) * REC;
         rec[4 + col] = O;
         if (col == 0) *reinterpret_cast<float4*>(rec) = make_float4(M, L, T, 0.f);
       }
@@ -1023,9 +1071,6 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
       }
     }
     __syncthreads();  // the shared rows are free again
-    rem += upto - from;
-    done += upto - from;
-    left -= upto - from;
   }
 }
 

