@@ -82,11 +82,13 @@ int run_chunk(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, 
   int e = allow_smem<paged_chunk_kernel<D, TIER>>(ChunkCfg<D>::kSmem);
   if (e != 0) return e;
   const unsigned n = static_cast<unsigned>(sm_count());
+  PagedJoin* joins = reinterpret_cast<PagedJoin*>(part);
+  part += kChunkJoinBytes / sizeof(float);
   e = launch_pdl(paged_chunk_kernel<D, TIER>, dim3(n), dim3(kChunkThreads), ChunkCfg<D>::kSmem, s, c, st, pl, q, heads,
-                 scale, out, ldo, H, part);
+                 scale, out, ldo, H, joins, part);
   if (e != 0) return e;
-  return launch_pdl(paged_join_kernel<D>, dim3(n, 8), dim3(256), 0, s, c, st, pl, heads, out, ldo, H,
-                    static_cast<const float*>(part));
+  return launch_pdl(paged_join_kernel<D>, dim3(n, 8), dim3(256), 0, s, pl, static_cast<const PagedJoin*>(joins), heads, out,
+                    ldo, H, static_cast<const float*>(part));
 }
 template <int D, int TIER>
 int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new, float scale,
@@ -117,7 +119,8 @@ int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& 
 size_t paged_head_bytes() { return 4096; }  // a ticket per CTA
 size_t paged_workspace_bytes(int64_t D) {
   // two parts per CTA: 16 rows of the few-row kernel's CTAs, 256 of the chunk kernel's
-  return paged_head_bytes() + size_t(2) * sm_count() * std::max<size_t>(few_ctas(1) * 16 * (D + 4), 256 * (D + 3)) * sizeof(float);
+  return paged_head_bytes() + size_t(2) * sm_count() * std::max<size_t>(few_ctas(1) * 16 * (D + 4), 256 * (D + 3)) * sizeof(float) +
+         kChunkJoinBytes;
 }
 
 #define EE_PAGED_DISPATCH(call)                                            \

@@ -572,8 +572,25 @@ __device__ __forceinline__ void paged_locate(const PagedArgs& c, const PagedStep
   b_out = st.batch;  // not reached while x < total
   rem = 0;
 }
-// CTA that holds cost x when W is dealt to n
-__device__ __forceinline__ int64_t paged_owner(int64_t x, int64_t W, int64_t n) { return ((x + 1) * n + W - 1) / W - 1; }
+// a / b for quotients below 2^20 or so, a >= 0, b > 0: the fp32 quotient is at most one off
+// (a 64-bit division takes several times as long, and the walk is on every part's way)
+__device__ __forceinline__ int64_t small_quotient(int64_t a, int64_t b) {
+  int64_t q = static_cast<int64_t>(__fdividef(static_cast<float>(a), static_cast<float>(b)));
+  int64_t r = a - q * b;
+  while (r < 0) {
+    --q;
+    r += b;
+  }
+  while (r >= b) {
+    ++q;
+    r -= b;
+  }
+  return q;
+}
+// CTA that holds cost x when W is dealt to n: the last with i W / n <= x
+__device__ __forceinline__ int64_t paged_owner(int64_t x, int64_t W, int64_t n) {
+  return small_quotient((x + 1) * n + W - 1, W) - 1;
+}
 
 // Where a CTA's share of the line stands.  paged_begin: by the whole block (share: three words of
 // shared memory); ncta: CTAs that have a share.
@@ -632,7 +649,7 @@ __device__ __forceinline__ bool paged_next(const PagedArgs& c, const PagedStepAr
       ++w.b;
       continue;
     }
-    const int64_t ch = w.rem / sc.chain;
+    const int64_t ch = small_quotient(w.rem, sc.chain);
     const int64_t at = w.rem - ch * sc.chain;  // cost from the chain's start
     int64_t lo = 0, hi = sc.chunks;            // the unit: the last with chain(lo) <= at
     while (hi - lo > 1) {

@@ -6,6 +6,7 @@
 // entropy, O += P V.  One CTA per SM, 512 threads:
 //   warps 0-1   UMMA issuers, one thread each, warp w for query tile w: S_0 | S_j+1, P_j V_j | ..
 //               (the next S runs under the softmax of the current one);
+//   warp 2      the walk over the CTA's share: hands the parts to the others;
 //   warps 4-7   the keys: a page's values come from HBM in the order they are kept, are
 //               converted to fp16 in registers (8-bit codes exactly: the scales stay out) and
 //               stored as the K-major SW128 operands K [128 keys, D] and V^T [D, 128 keys].  Each
@@ -33,7 +34,7 @@ namespace ee {
 constexpr int kChunkThreads = 512;
 // registers per thread at launch: 128 (512 threads, one CTA per SM), dealt out again by
 // warpgroup: issuers, keys, 2 x softmax
-constexpr int kChunkIssueRegs = 56, kChunkKeyRegs = 88, kChunkSoftmaxRegs = 184;
+constexpr int kChunkIssueRegs = 72, kChunkKeyRegs = 88, kChunkSoftmaxRegs = 176;
 static_assert(kChunkIssueRegs + kChunkKeyRegs + 2 * kChunkSoftmaxRegs <= 4 * 128, "register split above the launch budget");
 constexpr int kChunkTile = 128;                  // query rows per tile, keys per tile
 constexpr int kChunkBox = kChunkTile * 128;      // one SW128 block of 128 rows: 16 KB
@@ -46,7 +47,7 @@ struct ChunkCfg {
   static constexpr int kVBytes = 2 * D * 128;             // V^T: D rows, two blocks of 64 keys
   static constexpr int kPBytes = 2 * kChunkBox;
   static constexpr int NS = 2, NV = D == 64 ? 2 : 1;      // ring depths of K and V
-  static constexpr int kBarBytes = 256, kMetaBytes = kChunkMeta * 8 * 16;
+  static constexpr int kBarBytes = 512, kMetaBytes = kChunkMeta * 8 * 16;
   static constexpr size_t kSmem = 1024 + 2 * size_t(kQBytes) + NS * size_t(kQBytes) + NV * size_t(kVBytes) +
                                   2 * size_t(kPBytes) + kMetaBytes + kBarBytes;
   static_assert(kSmem <= 227 * 1024, "chunk attention above the 227 KB of shared memory per CTA");
@@ -78,23 +79,47 @@ __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence
 // any reference, but finite, so that 0 times their distance is 0
 constexpr float kMasked = -1e33f;
 
-// tiles of a part that query tile w takes part in
-template <int D>
-struct ChunkPart {
-  int n[2], nmax;  // key tiles of query tile 0 / 1, of the part
-  int tq;          // tokens of query tile 0
+// a unit that several CTAs share, as the CTA that begins it leaves it for the join
+struct PagedJoin {
+  int64_t row;      // query row of its first token
+  int h, hg, ntok;  // as in PagedPart
+  int cta0, cta1;   // the CTAs; equal: none
+  float vref;
+};
+constexpr size_t kChunkJoinBytes = 48 * 1024;  // room for the joins of 1024 CTAs
+static_assert(sizeof(PagedJoin) * 1024 <= kChunkJoinBytes, "room for the joins");
+
+// A part as the scheduling warp hands it to the others (through shared memory: the walk's 64-bit
+// state would cost every role the registers that its loop needs).
+struct __align__(16) ChunkJob {
+  int n[2], nmax, tile0;          // key tiles of query tile 0 / 1, of the part; the part's first (nmax < 0: no more)
+  int seq, h, hg, length;
+  int pos, ntok, row, whole;      // position of the unit's first token; tokens; its query row; all of the unit
+  float vref, log2_vref;
+  int first, pad;
 };
 __device__ __forceinline__ int chunk_tiles(int64_t reach) { return static_cast<int>((reach + kChunkTile - 1) / kChunkTile); }
-template <int D>
-__device__ __forceinline__ ChunkPart<D> chunk_part(const PagedPlan& pl, const PagedPart& u) {
-  ChunkPart<D> p;
+__device__ __forceinline__ ChunkJob chunk_job(const PagedArgs& c, const PagedPlan& pl, const PagedPart& u) {
+  ChunkJob p;
   const int half = pl.TQ / 2;
-  p.tq = u.ntok < half ? u.ntok : half;
-  const int t0 = chunk_tiles(u.s.start + u.tok0 + p.tq);
+  const int t0 = chunk_tiles(u.s.start + u.tok0 + (u.ntok < half ? u.ntok : half));
   const int e0 = t0 < u.tile1 ? t0 : u.tile1;
   p.n[0] = e0 > u.tile0 ? e0 - u.tile0 : 0;
   p.n[1] = u.ntok > half && u.tile1 > u.tile0 ? u.tile1 - u.tile0 : 0;
   p.nmax = p.n[0] > p.n[1] ? p.n[0] : p.n[1];
+  p.tile0 = u.tile0;
+  p.seq = static_cast<int>(u.s.seq);
+  p.h = u.h;
+  p.hg = u.hg;
+  p.length = static_cast<int>(u.s.length);
+  p.pos = static_cast<int>(u.s.start + u.tok0);
+  p.ntok = u.ntok;
+  p.row = static_cast<int>(u.s.row0 + u.tok0);
+  p.whole = u.whole;
+  p.first = u.first;
+  p.vref = paged_vref(c, u.s, u.h);
+  p.log2_vref = __log2f(p.vref);
+  p.pad = 0;
   return p;
 }
 
@@ -102,7 +127,7 @@ template <int D, int TIER>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     paged_chunk_kernel(const PagedArgs c, const PagedStepArgs st, const PagedPlan pl, const PagedRows q, int heads,
                        float scale, __half* __restrict__ out, int64_t ldo, float* __restrict__ H,
-                       float* __restrict__ part) {
+                       PagedJoin* __restrict__ joins, float* __restrict__ part) {
   using Cfg = ChunkCfg<D>;
   constexpr int NS = Cfg::NS, NV = Cfg::NV, T = kChunkTile;
   extern __shared__ uint8_t chunk_smem[];
@@ -124,10 +149,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* o_done = p_full + 2;      // [2] P_w V done
   uint64_t* o_free = o_done + 2;      // [2] O_w read out (4 warps)
   uint64_t* drain = o_free + 2;       // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+  uint64_t* job_full = drain + 2;     // [2] a job handed out
+  uint64_t* job_empty = job_full + 2; // [2] read by the 14 other warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(job_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int64_t* s_share = reinterpret_cast<int64_t*>(tmem_slot + 2);
-  static_assert((2 + 2 * NS + 2 * NV + 12) * 8 + 8 + 24 <= Cfg::kBarBytes, "barrier region overflows");
+  ChunkJob* jobs = reinterpret_cast<ChunkJob*>(reinterpret_cast<uint8_t*>(bars) + Cfg::kBarBytes - 2 * sizeof(ChunkJob));
+  static_assert((2 + 2 * NS + 2 * NV + 16) * 8 + 8 + 24 + 2 * sizeof(ChunkJob) <= Cfg::kBarBytes, "barrier region overflows");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -147,12 +175,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 4);
       mbar_init(&drain[i], 1);
+      mbar_init(&job_full[i], 1);
+      mbar_init(&job_empty[i], 14);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   griddep_wait();
   PagedWalk walk = paged_begin(c, st, pl, blockIdx.x, gridDim.x, s_share);
+  if (threadIdx.x == 64) joins[blockIdx.x] = PagedJoin{};  // (the scheduling warp's lane 0 fills it)
   if (walk.left <= 0) return;
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -169,10 +200,42 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
   };
 
-  PagedPart u;
+  // the next job, for every warp but the scheduling one: a copy of the fields it names
+  uint32_t njob = 0;
+  ChunkJob u;
+  auto next_job = [&]() -> bool {
+    const int i = njob & 1;
+    if (!mbar_wait_warp(&job_full[i], (njob >> 1) & 1u, abort_flag)) return false;
+    u = jobs[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&job_empty[i]);
+    ++njob;
+    return true;
+  };
   if (warp < 4) {
     warpgroup_reg_dealloc<kChunkIssueRegs>();
-    if (warp < 2) {
+    if (warp == 2) {
+      // ------------------------------------------------------------ the walk
+      PagedPart part_u;
+      bool ok = true, more = true;
+      for (uint32_t k = 0; ok && more; ++k) {
+        more = paged_next<T>(c, st, pl, walk, part_u);
+        ChunkJob job = {};
+        job.nmax = -1;
+        if (more) job = chunk_job(c, pl, part_u);
+        ok = mbar_wait_warp(&job_empty[k & 1], ((k >> 1) & 1u) ^ 1u, abort_flag);
+        if (!ok) break;
+        if (lane == 0) {
+          jobs[k & 1] = job;
+          mbar_arrive(&job_full[k & 1]);
+          if (more && part_u.first && !part_u.whole)
+            joins[blockIdx.x] = PagedJoin{part_u.s.row0 + part_u.tok0, part_u.h, part_u.hg, part_u.ntok,
+                                          static_cast<int>(part_u.cta0), static_cast<int>(part_u.cta1), job.vref};
+        }
+        __syncwarp();
+      }
+      if (!ok) give_up();
+    } else if (warp < 2) {
       // ------------------------------------------------------------ UMMA issuers
       constexpr uint32_t idesc_s = make_idesc(1u, 0u, T, T);
       constexpr uint32_t idesc_o = make_idesc(1u, 0u, T, D);
@@ -218,12 +281,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         __syncwarp();
         return true;
       };
-      while (ok && paged_next<T>(c, st, pl, walk, u)) {
-        const ChunkPart<D> cp = chunk_part<D>(pl, u);
-        const int n = cp.n[w];
+      while (ok) {
+        ok = next_job();
+        if (!ok || u.nmax < 0) break;
+        const int n = w ? u.n[1] : u.n[0];
         if (n > 0) ok = mbar_wait_warp(&q_full[w], loads & 1u, abort_flag);
-        for (int j = -1; ok && j < cp.nmax; ++j) {
-          if (j + 1 < cp.nmax) {  // S of tile j + 1 (or its share of the K stage's release)
+        for (int j = -1; ok && j < u.nmax; ++j) {
+          if (j + 1 < u.nmax) {  // S of tile j + 1 (or its share of the K stage's release)
             const uint32_t kn = kt + j + 1;
             ok = j + 1 < n ? issue_s(kn, g + j + 1) : mbar_wait_warp(&k_full[kn % NS], (kn / NS) & 1u, abort_flag);
             if (ok && lane == 0) tc_commit(&k_empty[kn % NS]);
@@ -242,8 +306,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             __syncwarp();
           }
         }
-        kt += cp.nmax;
-        vt += cp.nmax;
+        kt += u.nmax;
+        vt += u.nmax;
         g += n;
         loads += n > 0;
       }
@@ -271,162 +335,201 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     auto v_at = [&](uint8_t* tile, int i) -> uint4* {  // dimension gq D/8 + i
       return reinterpret_cast<uint4*>(tile + (kw >> 1) * (D * 128) + (8 * i + gq) * 128 + (((2 * q4 + (kw & 1)) ^ gq) << 4));
     };
-    while (ok && paged_next<T>(c, st, pl, walk, u)) {
-      const ChunkPart<D> cp = chunk_part<D>(pl, u);
-      const PagedSeq& s = u.s;
-      const int64_t full = TIER == kFP16 ? c.max_pages : s.length >> c.page_shift;  // blocks in pages
-      const int32_t* table = c.table + s.seq * c.max_pages;
-      const float log2_vref = __log2f(paged_vref(c, s, u.h));
-      // where a group's values are: nowhere (a hole, or past the tokens), in a page, in the open block
-      auto lookup = [&](int j, int (&pgs)[2]) {
+    // x: eight or fewer 16-byte units of each of the two groups.  An item (K or V of a tile) takes
+    // kHalves rounds of x; a unit is refilled for the next round as soon as it is used.
+    constexpr bool kWide = TIER == kFP16;
+    constexpr int kHalves = kWide && D == 128 ? 2 : 1;
+    constexpr int kUnits = (kWide ? D / 16 : D / 32) / kHalves;  // per group and round
+    constexpr int kCodes = kWide ? kINT8 : TIER;
+    uint4 x[2][kUnits];
+    while (ok) {
+      ok = next_job();
+      if (!ok || u.nmax < 0) break;
+      if (u.nmax == 0) continue;
+      const int full = kWide ? INT_MAX : u.length >> c.page_shift;  // blocks in pages
+      const int ends = (u.length + 15) >> 4;                        // groups with tokens
+      const int32_t* table = c.table + u.seq * c.max_pages;
+      const float log2_vref = u.log2_vref;
+      const int gbase = u.tile0 * 8 + 2 * kw;  // this warp's first group of tile 0 of the part
+      // where a group's values are: nowhere (-1: a hole, or past the tokens), page p, the open block
+      struct Pages {
+        int p[2];
+      };
+      auto lookup = [&](int j) -> Pages {
+        Pages r;
 #pragma unroll
         for (int ga = 0; ga < 2; ++ga) {
-          const int64_t g = static_cast<int64_t>(u.tile0 + j) * 8 + 2 * kw + ga, blk = g >> pg;
+          const int g = gbase + 8 * j + ga, blk = g >> pg;
           int p = -1;
-          if (j < cp.nmax && g * 16 < s.length) {
+          if (j < u.nmax && g < ends) {
             if (blk >= full) {
-              p = INT_MAX;  // open
+              p = INT_MAX;
             } else {
-              p = table[blk];
+              p = __ldg(table + blk);
               p = p >= 0 && p < c.num_pages ? p : -1;
             }
           }
-          pgs[ga] = p;
+          r.p[ga] = p;
         }
+        return r;
       };
-      auto meta_of = [&](int p) -> float4 {
-        if (p < 0) return make_float4(1e-25f, kMasked, 1.f, 0.f);
-        float2 sc = make_float2(1.f, 1.f);
-        if (TIER != kFP16 && p != INT_MAX)
-          sc = *reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2);
-        const float lv = v_shift(sc.y, log2_vref);
-        return make_float4(fmaxf(to2 * sc.x, 1e-25f), lv, ex2_approx(-lv), 0.f);
+      // a group's first unit of this lane (K: which 0, V: 1), null where nothing is prefetched
+      auto source = [&](const Pages& r, int j, int which, int ga) -> const uint4* {
+        const int g = (gbase + 8 * j + ga) & ((1 << pg) - 1);
+        if (r.p[ga] < 0 || r.p[ga] == INT_MAX) return nullptr;
+        return reinterpret_cast<const uint4*>(paged_block(c, r.p[ga], u.h, which)) + g * (kWide ? 2 * D : D) + lane;
       };
-      for (int j = -1; ok && j < cp.nmax; ++j) {
-        // K of tile j + 1, then V of tile j
-        const bool k_now = j + 1 < cp.nmax;
-        for (int which = 0; which < 2 && ok; ++which) {
-          if (which == 0 ? !k_now : j < 0) continue;
-          const int tile_j = which == 0 ? j + 1 : j;
-          int pgs[2];
-          lookup(tile_j, pgs);
-          const uint32_t idx = which == 0 ? kt + tile_j : vt + tile_j;
-          const int stage = which == 0 ? idx % NS : idx % NV;
-          uint64_t* empty = which == 0 ? &k_empty[stage] : &v_empty[stage];
-          const uint32_t par = ((which == 0 ? idx / NS : idx / NV) & 1u) ^ 1u;
-          uint8_t* dst = which == 0 ? sK + stage * Cfg::kQBytes : sV + stage * Cfg::kVBytes;
-          const int64_t g0 = static_cast<int64_t>(u.tile0 + tile_j) * 8 + 2 * kw;
-          const bool wide0 = TIER == kFP16 || pgs[0] == INT_MAX, wide1 = TIER == kFP16 || pgs[1] == INT_MAX;
-          auto base = [&](int ga) -> const uint8_t* {
-            const int64_t g = g0 + ga, off = (g & ((1 << pg) - 1)) * 16 * D;
-            if (pgs[ga] == INT_MAX)
-              return reinterpret_cast<const uint8_t*>(paged_open(c, s.seq, full, u.h, which) + off) + lane * 16;
-            return paged_block(c, pgs[ga], u.h, which) + off * (TIER == kFP16 ? 2 : 1) + lane * 16;
-          };
-          if (which == 0) {
-            float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (lane < 2) m = meta_of(lane == 0 ? pgs[0] : pgs[1]);
-            uint4 x[2][D / 32];
-            if constexpr (TIER != kFP16) {
+      auto open_source = [&](int j, int which, int ga) -> const uint4* {
+        const int g = (gbase + 8 * j + ga) & ((1 << pg) - 1);
+        return reinterpret_cast<const uint4*>(paged_open(c, u.seq, full, u.h, which)) + g * 2 * D + lane;
+      };
+      auto fetch = [](const uint4* src, int i) -> uint4 { return src ? __ldg(src + 32 * i) : make_uint4(0, 0, 0, 0); };
+      auto scales = [&](const Pages& r) -> float2 {  // lanes 0, 1: of their group
+        const int p = lane == 0 ? r.p[0] : r.p[1];
+        if (kWide || lane > 1 || p < 0 || p == INT_MAX) return make_float2(1.f, 1.f);
+        return __ldg(reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2));
+      };
+      auto zero_code = [](uint4 v, bool there) -> uint4 {  // a hole's codes stand for zeros
+        if (kWide || TIER != kINT8 || there) return v;
+        return make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+      };
+
+      // the item after the one in x: its sources
+      const uint4* nsrc[2];
+      auto aim = [&](const Pages& r, int j, int which) {
+        nsrc[0] = source(r, j, which, 0);
+        nsrc[1] = source(r, j, which, 1);
+      };
+      auto k_item = [&](const Pages& r, int j, float2 sc) {  // stores K of tile j from x, refills x from nsrc
+        const uint32_t idx = kt + j;
+        const int stage = idx % NS;
+        ok = mbar_wait_warp(&k_empty[stage], ((idx / NS) & 1u) ^ 1u, abort_flag);
+        if (!ok) return;
+        uint8_t* dst = sK + stage * Cfg::kQBytes;
+        if (lane < 2) {
+          const int p = lane == 0 ? r.p[0] : r.p[1];
+          const float lv = v_shift(sc.y, log2_vref);
+          sMeta[(idx % kChunkMeta) * 8 + 2 * kw + lane] =
+              p < 0 ? make_float4(1e-25f, kMasked, 1.f, 0.f) : make_float4(fmaxf(to2 * sc.x, 1e-25f), lv, ex2_approx(-lv), 0.f);
+        }
+        const uint4* own[2] = {source(r, j, 0, 0), source(r, j, 0, 1)};
 #pragma unroll
-              for (int ga = 0; ga < 2; ++ga)
+        for (int hh = 0; hh < kHalves; ++hh) {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-                  x[ga][i] = pgs[ga] >= 0 && !(ga ? wide1 : wide0)
-                                 ? __ldg(reinterpret_cast<const uint4*>(base(ga) + i * 512))
-                                 : make_uint4(0, 0, 0, 0);
-            }
-            ok = mbar_wait_warp(empty, par, abort_flag);
-            if (!ok) break;
-            if (lane < 2) sMeta[(idx % kChunkMeta) * 8 + 2 * kw + lane] = m;
+          for (int ga = 0; ga < 2; ++ga) {
+            const uint4* refill = hh + 1 < kHalves ? own[ga] : nsrc[ga];
+            if (!kWide && r.p[ga] == INT_MAX) {  // the open block's fp16 rows
+              const uint4* src = open_source(j, 0, ga);
 #pragma unroll
-            for (int ga = 0; ga < 2; ++ga) {
-              if (ga ? wide1 : wide0) {
-                const uint4* src = reinterpret_cast<const uint4*>(pgs[ga] >= 0 ? base(ga) : nullptr);
+              for (int i = 0; i < D / 16; ++i) *k_at(dst, ga, i / (D / 32), (i % (D / 32)) >> 1, i & 1) = __ldg(src + 32 * i);
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i) {
-                  const uint4 y = pgs[ga] >= 0 ? src[i * 32] : make_uint4(0, 0, 0, 0);
-                  const int hf = i / (D / 32), p8 = i % (D / 32);
-                  *k_at(dst, ga, hf, p8 >> 1, p8 & 1) = y;
-                }
-              } else if constexpr (TIER != kFP16) {
+              for (int i = 0; i < kUnits; ++i) x[ga][i] = fetch(refill, i);
+            } else {
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                  const int hf = i / (D / 64), piece = i % (D / 64);
-                  uint4 a, b;
-                  if (pgs[ga] >= 0) {
-                    codes_to_h2<TIER>(x[ga][i].x, a.x, a.y);
-                    codes_to_h2<TIER>(x[ga][i].y, a.z, a.w);
-                    codes_to_h2<TIER>(x[ga][i].z, b.x, b.y);
-                    codes_to_h2<TIER>(x[ga][i].w, b.z, b.w);
-                  } else {
-                    a = b = make_uint4(0, 0, 0, 0);
-                  }
-                  *k_at(dst, ga, hf, piece, 0) = a;
-                  *k_at(dst, ga, hf, piece, 1) = b;
-                }
-              }
-            }
-          } else {
-            uint4 x[2][D / 32];
-            if constexpr (TIER != kFP16) {
-#pragma unroll
-              for (int ga = 0; ga < 2; ++ga)
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i)
-                  x[ga][i] = pgs[ga] >= 0 && !(ga ? wide1 : wide0)
-                                 ? __ldg(reinterpret_cast<const uint4*>(base(ga) + i * 512))
-                                 : make_uint4(0, 0, 0, 0);
-            }
-            ok = mbar_wait_warp(empty, par, abort_flag);
-            if (!ok) break;
-            uint32_t keep[2][2];  // tokens past the sequence's are no numbers to multiply by
-#pragma unroll
-            for (int ga = 0; ga < 2; ++ga)
-#pragma unroll
-              for (int th = 0; th < 2; ++th) {
-                const int64_t t0 = (g0 + ga) * 16 + 2 * q4 + 8 * th;
-                keep[ga][th] = pgs[ga] < 0 ? 0u : ((t0 < s.length ? 0xffffu : 0u) | (t0 + 1 < s.length ? 0xffff0000u : 0u));
-              }
-            const uint8_t* b0 = pgs[0] >= 0 ? base(0) : nullptr;
-            const uint8_t* b1 = pgs[1] >= 0 ? base(1) : nullptr;
-#pragma unroll
-            for (int mb = 0; mb < D / 16; ++mb) {
-              uint4 lo, hi;  // dimensions 2 mb, 2 mb + 1: keys of group 0 (two pairs), of group 1
-#pragma unroll
-              for (int ga = 0; ga < 2; ++ga) {
-                uint32_t j0t0, j1t0, j0t1, j1t1;
-                if (ga ? wide1 : wide0) {
-                  const uint4 y = pgs[ga] >= 0 ? reinterpret_cast<const uint4*>(ga ? b1 : b0)[mb * 32] : make_uint4(0, 0, 0, 0);
-                  j0t0 = y.x;
-                  j1t0 = y.y;
-                  j0t1 = y.z;
-                  j1t1 = y.w;
+              for (int i = 0; i < kUnits; ++i) {
+                if constexpr (kWide) {
+                  const int k = hh * kUnits + i;
+                  *k_at(dst, ga, k / (D / 32), (k % (D / 32)) >> 1, k & 1) = x[ga][i];
                 } else {
-                  const uint4 y = x[ga][TIER != kFP16 ? mb >> 1 : 0];
-                  codes_to_h2<TIER == kFP16 ? kINT8 : TIER>(mb & 1 ? y.z : y.x, j0t0, j1t0);
-                  codes_to_h2<TIER == kFP16 ? kINT8 : TIER>(mb & 1 ? y.w : y.y, j0t1, j1t1);
+                  const uint4 v = zero_code(x[ga][i], r.p[ga] >= 0);
+                  uint4 a, b;
+                  codes_to_h2<kCodes>(v.x, a.x, a.y);
+                  codes_to_h2<kCodes>(v.y, a.z, a.w);
+                  codes_to_h2<kCodes>(v.z, b.x, b.y);
+                  codes_to_h2<kCodes>(v.w, b.z, b.w);
+                  *k_at(dst, ga, i / (D / 64), i % (D / 64), 0) = a;
+                  *k_at(dst, ga, i / (D / 64), i % (D / 64), 1) = b;
                 }
-                j0t0 &= keep[ga][0];
-                j1t0 &= keep[ga][0];
-                j0t1 &= keep[ga][1];
-                j1t1 &= keep[ga][1];
-                (ga ? lo.z : lo.x) = j0t0;
-                (ga ? lo.w : lo.y) = j0t1;
-                (ga ? hi.z : hi.x) = j1t0;
-                (ga ? hi.w : hi.y) = j1t1;
+                x[ga][i] = fetch(refill, (hh + 1 < kHalves ? (hh + 1) * kUnits : 0) + i);
               }
-              *v_at(dst, 2 * mb) = lo;
-              *v_at(dst, 2 * mb + 1) = hi;
             }
           }
-          fence_proxy_async_shared();  // the stores, visible to the tensor core
-          __syncwarp();
-          if (lane == 0) mbar_arrive(which == 0 ? &k_full[stage] : &v_full[stage]);
         }
+        fence_proxy_async_shared();  // the stores, visible to the tensor core
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&k_full[stage]);
+      };
+      auto v_item = [&](const Pages& r, int j) {
+        const uint32_t idx = vt + j;
+        const int stage = idx % NV;
+        ok = mbar_wait_warp(&v_empty[stage], ((idx / NV) & 1u) ^ 1u, abort_flag);
+        if (!ok) return;
+        uint8_t* dst = sV + stage * Cfg::kVBytes;
+        const bool open0 = !kWide && r.p[0] == INT_MAX, open1 = !kWide && r.p[1] == INT_MAX;
+        const uint4* own[2] = {source(r, j, 1, 0), source(r, j, 1, 1)};
+        uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};  // tokens past the sequence's are no numbers to multiply by
+        if (kWide || open0 || open1) {
+#pragma unroll
+          for (int ga = 0; ga < 2; ++ga)
+#pragma unroll
+            for (int th = 0; th < 2; ++th) {
+              const int t0 = (gbase + 8 * j + ga) * 16 + 2 * q4 + 8 * th;
+              keep[ga][th] = (t0 < u.length ? 0xffffu : 0u) | (t0 + 1 < u.length ? 0xffff0000u : 0u);
+            }
+        }
+        const uint4* os[2] = {open0 ? open_source(j, 1, 0) : nullptr, open1 ? open_source(j, 1, 1) : nullptr};
+#pragma unroll
+        for (int hh = 0; hh < kHalves; ++hh) {
+#pragma unroll
+          for (int m = 0; m < D / 16 / kHalves; ++m) {
+            const int mb = hh * (D / 16 / kHalves) + m, i = kWide ? m : m >> 1;
+            uint32_t j0[4], j1[4];  // dimensions 2 mb, 2 mb + 1: two pairs of keys of group 0, of group 1
+#pragma unroll
+            for (int ga = 0; ga < 2; ++ga) {
+              if (kWide || (ga ? open1 : open0)) {
+                const uint4 y = kWide ? x[ga][i] : __ldg(os[ga] + 32 * mb);
+                j0[2 * ga] = y.x & keep[ga][0];
+                j1[2 * ga] = y.y & keep[ga][0];
+                j0[2 * ga + 1] = y.z & keep[ga][1];
+                j1[2 * ga + 1] = y.w & keep[ga][1];
+              } else {
+                const uint4 v = zero_code(x[ga][i], r.p[ga] >= 0);
+                codes_to_h2<kCodes>(m & 1 ? v.z : v.x, j0[2 * ga], j1[2 * ga]);
+                codes_to_h2<kCodes>(m & 1 ? v.w : v.y, j0[2 * ga + 1], j1[2 * ga + 1]);
+              }
+            }
+            *v_at(dst, 2 * mb) = make_uint4(j0[0], j0[1], j0[2], j0[3]);
+            *v_at(dst, 2 * mb + 1) = make_uint4(j1[0], j1[1], j1[2], j1[3]);
+            if (kWide || (m & 1)) {
+#pragma unroll
+              for (int ga = 0; ga < 2; ++ga)
+                x[ga][i] = fetch(hh + 1 < kHalves ? own[ga] : nsrc[ga], (hh + 1 < kHalves ? (hh + 1) * kUnits : 0) + i);
+            }
+          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_full[stage]);
+      };
+
+      // K_0 | K_1 V_0 | K_2 V_1 | ..; page numbers a tile ahead of the loads that need them
+      Pages p0 = lookup(0), p1 = lookup(1);
+      float2 sc = scales(p0);
+      aim(p0, 0, 0);
+#pragma unroll
+      for (int ga = 0; ga < 2; ++ga)
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) x[ga][i] = fetch(nsrc[ga], i);
+      float2 sc1 = scales(p1);
+      if (u.nmax > 1) aim(p1, 1, 0);
+      else aim(p0, 0, 1);
+      k_item(p0, 0, sc);
+      for (int j = 0; ok && j < u.nmax; ++j) {  // x: K of tile j + 1, or V of tile j if it is the last
+        const Pages p2 = lookup(j + 2);
+        if (j + 1 < u.nmax) {
+          aim(p0, j, 1);
+          k_item(p1, j + 1, sc1);
+          if (!ok) break;
+        }
+        sc1 = scales(p2);
+        if (j + 2 < u.nmax) aim(p2, j + 2, 0);
+        else aim(p1, j + 1, 1);  // past the last tile: p1 holds nothing, and nothing is loaded
+        v_item(p0, j);
+        p0 = p1;
+        p1 = p2;
       }
-      kt += cp.nmax;
-      vt += cp.nmax;
+      kt += u.nmax;
+      vt += u.nmax;
     }
     if (!ok) give_up();
   } else {
@@ -441,23 +544,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const int rx = row & 7;
     bool ok = true;
     uint32_t kt = 0, g = 0;
-    while (ok && paged_next<T>(c, st, pl, walk, u)) {
-      const ChunkPart<D> cp = chunk_part<D>(pl, u);
-      const int n = cp.n[w];
+    while (ok) {
+      ok = next_job();
+      if (!ok || u.nmax < 0) break;
+      const int n = w ? u.n[1] : u.n[0];
       // this row: token and query head
       const int half = pl.TQ / 2, tok = row / pl.Gc + w * half, hd = u.hg * pl.Gc + row % pl.Gc;
       const bool real = row < half * pl.Gc && tok < u.ntok && hd < pl.G;
-      const int64_t qrow = u.s.row0 + u.tok0 + (real ? tok : 0);
+      const int64_t qrow = u.row + (real ? tok : 0);
       const int head = u.h * pl.G + (real ? hd : 0);
       float m = kNegInf, l = 0.f, t = 0.f;
       if (n > 0) {
         // Q: the S MMAs of the part before have read the old one (their last S was waited for)
         const uint4* src = reinterpret_cast<const uint4*>(q.p + qrow * q.ld + head * D);
+        uint4 x[D / 8];  // all loads before the first store
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) x[i] = real ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-          const uint4 x = real ? src[i] : make_uint4(0, 0, 0, 0);
           const int q4 = i / (D / 32), r = i % (D / 32);  // dimensions 8 i ..: piece r / 2, chunk 2 q4 + r % 2
-          *reinterpret_cast<uint4*>(qbuf + (r >> 1) * kChunkBox + (((2 * q4 + (r & 1)) ^ rx) << 4)) = x;
+          *reinterpret_cast<uint4*>(qbuf + (r >> 1) * kChunkBox + (((2 * q4 + (r & 1)) ^ rx) << 4)) = x[i];
         }
         fence_proxy_async_shared();
         __syncwarp();
@@ -468,9 +574,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         ok = mbar_wait_warp(&s_full[w], gj & 1u, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        const int64_t key0 = static_cast<int64_t>(u.tile0 + j) * T;
-        const int64_t seen = u.s.start + u.tok0 + tok + 1 - key0;
-        const int lim = !real || seen > T ? T : (seen < 0 ? 0 : static_cast<int>(seen));
+        const int seen = u.pos + tok + 1 - (u.tile0 + j) * T;
+        const int lim = !real || seen > T ? T : (seen < 0 ? 0 : seen);
         uint32_t r[4][32];
         __syncwarp();
 #pragma unroll
@@ -570,8 +675,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       float* rec = part + (2 * static_cast<int64_t>(blockIdx.x) + (u.first ? 1 : 0)) * Cfg::kRec + w * T + row;
       if (n > 0) {
         tc_fence_after();
-        const float vref = paged_vref(c, u.s, u.h);
-        const float f = l != 0.f ? vref / l : 0.f;  // a row that sees no key: zeros
+        const float f = l != 0.f ? u.vref / l : 0.f;  // a row that sees no key: zeros
         __half* dst = out + qrow * ldo + head * D;
 #pragma unroll
         for (int hh = 0; hh < D / 64; ++hh) {  // columns 64 hh ..: dimensions 8 hh .. of each gq's
@@ -595,7 +699,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 *reinterpret_cast<uint4*>(dst + gq * (D / 8) + 8 * hh) = make_uint4(o[0], o[1], o[2], o[3]);
               }
             }
-          } else {
+          } else if (real) {
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               rec[(3 + 64 * hh + k) * 256] = __uint_as_float(a[k]);
@@ -612,12 +716,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (real && n == 0) {
           for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(out + qrow * ldo + head * D + 8 * i) = make_uint4(0, 0, 0, 0);
         }
-      } else {
+      } else if (real) {
         rec[0] = m;
         rec[256] = l;
         rec[512] = t;
       }
-      kt += cp.nmax;
+      kt += u.nmax;
       g += n;
     }
     if (!ok) give_up();
@@ -630,49 +734,47 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 }
 
 // The units that several CTAs shared: block (x, y) joins rows 32 y .. of the unit that begins in CTA
-// x's share and runs past it, its parts in the order of the keys.  Warp gq sums the dimensions
-// gq D/8 .. of a row per lane.
+// x's share and runs past it (joins[x], written by that CTA), its parts in the order of the
+// keys.  Warp gq sums the dimensions gq D/8 .. of a row per lane: every load is a full line, and
+// none waits for another but the first (l and m say whether O was written at all, and then
+// select, not branch).
 template <int D>
 __global__ void __launch_bounds__(256)
-    paged_join_kernel(const PagedArgs c, const PagedStepArgs st, const PagedPlan pl, int heads, __half* __restrict__ out,
+    paged_join_kernel(const PagedPlan pl, const PagedJoin* __restrict__ joins, int heads, __half* __restrict__ out,
                       int64_t ldo, float* __restrict__ H, const float* __restrict__ part) {
   using Cfg = ChunkCfg<D>;
-  __shared__ int64_t s_share[3];
   griddep_wait();
   griddep_launch_dependents();
-  PagedWalk walk = paged_begin(c, st, pl, blockIdx.x, gridDim.x, s_share);
-  PagedPart u;
-  bool found = false;
-  while (paged_next<kChunkTile>(c, st, pl, walk, u))
-    if (u.first && !u.whole) {
-      found = true;
-      break;
-    }
-  if (!found) return;
+  const PagedJoin u = joins[blockIdx.x];
+  if (u.cta1 <= u.cta0) return;
   const int lane = threadIdx.x & 31, gq = threadIdx.x >> 5;
   const int r = blockIdx.y * 32 + lane, w = r >> 7, row = r & 127;
   const int half = pl.TQ / 2, tok = row / pl.Gc + w * half, hd = u.hg * pl.Gc + row % pl.Gc;
-  const bool real = row < half * pl.Gc && tok < u.ntok && hd < pl.G;
-  if (!real) return;
-  auto rec_of = [&](int64_t k) { return part + (2 * k + (k == u.cta0 ? 1 : 0)) * Cfg::kRec + r; };
+  if (row >= half * pl.Gc || tok >= u.ntok || hd >= pl.G) return;
+  auto rec_of = [&](int k) { return part + (2 * static_cast<int64_t>(k) + (k == u.cta0 ? 1 : 0)) * Cfg::kRec + r; };
   float M = kNegInf;
-  for (int64_t k = u.cta0; k <= u.cta1; ++k) M = fmaxf(M, rec_of(k)[0]);
+#pragma unroll 4
+  for (int k = u.cta0; k <= u.cta1; ++k) M = fmaxf(M, rec_of(k)[0]);
   float L = 0.f, T = 0.f, o[D / 8];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) o[i] = 0.f;
-  for (int64_t k = u.cta0; k <= u.cta1; ++k) {
+#pragma unroll 2
+  for (int k = u.cta0; k <= u.cta1; ++k) {
     const float* rec = rec_of(k);
-    const float m = rec[0], l = rec[256];
-    if (m == kNegInf && l == 0.f) continue;  // a part that saw no key of the row
-    const float a = m == kNegInf ? 1.f : ex2_approx(m - M);
-    L = fmaf(a, l, L);
-    T = fmaf(a, rec[512] + (m == kNegInf ? 0.f : l * (m - M)), T);
+    const float m = rec[0], l = rec[256], t = rec[512];
+    float x[D / 8];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i] = fmaf(a, rec[(3 + 8 * i + gq) * 256], o[i]);
+    for (int i = 0; i < D / 8; ++i) x[i] = rec[(3 + 8 * i + gq) * 256];
+    const bool none = m == kNegInf && l == 0.f;  // a part that saw no key of the row
+    const float a = none ? 0.f : (m == kNegInf ? 1.f : ex2_approx(m - M));
+    L = fmaf(a, l, L);
+    T = none ? T : fmaf(a, t + (m == kNegInf ? 0.f : l * (m - M)), T);
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i] = none ? o[i] : fmaf(a, x[i], o[i]);
   }
-  const int64_t qrow = u.s.row0 + u.tok0 + tok;
+  const int64_t qrow = u.row + tok;
   const int head = u.h * pl.G + hd;
-  const float f = L != 0.f ? paged_vref(c, u.s, u.h) / L : 0.f;
+  const float f = L != 0.f ? u.vref / L : 0.f;
 #pragma unroll
   for (int i = 0; i < D / 8; i += 8) {
     uint32_t x[4];
