@@ -7,11 +7,10 @@
 //   warps 0-1   UMMA issuers, one thread each, warp w for query tile w: S_0 | S_j+1, P_j V_j | ..
 //               (the next S runs under the softmax of the current one);
 //   warp 2      the walk over the CTA's share: hands the parts to the others;
-//   warps 4-7   the keys: a page's values come from HBM in the order they are kept, are
-//               converted to fp16 in registers (8-bit codes exactly: the scales stay out) and
-//               stored as the K-major SW128 operands K [128 keys, D] and V^T [D, 128 keys].  Each
-//               unit of 16 bytes is replaced by the next tile's as soon as it is used, so a
-//               tile's loads are in flight during the tile before;
+//   warp 3      bulk copies of the pages' values, 16 KB a round, a tile ahead;
+//   warps 4-7   the keys: a round's values are converted to fp16 in registers (8-bit codes
+//               exactly: the scales stay out) and stored as the K-major SW128 operands
+//               K [128 keys, D] and V^T [D, 128 keys];
 //   warps 8-15  warpgroup w = query tile w, one row per thread: scores from TMEM, row
 //               maximum, P = 2^(x - m) as fp16 into shared memory, l and t, and at the end
 //               O / l (or the part's O, l, t, m for the join).
@@ -38,7 +37,7 @@ constexpr int kChunkIssueRegs = 72, kChunkKeyRegs = 88, kChunkSoftmaxRegs = 176;
 static_assert(kChunkIssueRegs + kChunkKeyRegs + 2 * kChunkSoftmaxRegs <= 4 * 128, "register split above the launch budget");
 constexpr int kChunkTile = 128;                  // query rows per tile, keys per tile
 constexpr int kChunkBox = kChunkTile * 128;      // one SW128 block of 128 rows: 16 KB
-constexpr int kChunkMeta = 4;                    // tiles of scales held
+constexpr int kChunkMeta = 8;                    // tiles of scales held
 
 template <int D>
 struct ChunkCfg {
@@ -46,10 +45,12 @@ struct ChunkCfg {
   static constexpr int kQBytes = KB * kChunkBox;          // a Q tile, a K tile
   static constexpr int kVBytes = 2 * D * 128;             // V^T: D rows, two blocks of 64 keys
   static constexpr int kPBytes = 2 * kChunkBox;
-  static constexpr int NS = 2, NV = D == 64 ? 2 : 1;      // ring depths of K and V
+  static constexpr int NS = D == 64 ? 2 : 1, NV = NS;     // ring depths of K and V
+  // rounds of a tile's K or V as it is kept: 16 KB (fp16 with D = 128: two rounds)
+  static constexpr int NR = 2, kRawBytes = 16 * 1024;
   static constexpr int kBarBytes = 512, kMetaBytes = kChunkMeta * 8 * 16;
   static constexpr size_t kSmem = 1024 + 2 * size_t(kQBytes) + NS * size_t(kQBytes) + NV * size_t(kVBytes) +
-                                  2 * size_t(kPBytes) + kMetaBytes + kBarBytes;
+                                  2 * size_t(kPBytes) + NR * size_t(kRawBytes) + kMetaBytes + kBarBytes;
   static_assert(kSmem <= 227 * 1024, "chunk attention above the 227 KB of shared memory per CTA");
   static constexpr uint32_t kTmemS = 0, kTmemO = 2 * kChunkTile;
   // a part's results: (m, l, t, then the D columns in V^T's row order) x 256 rows
@@ -75,6 +76,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// where a group of 16 keys is, besides page p >= 0: nowhere (a hole, or past the tokens), in the open block
+constexpr int kNowhere = -1, kOpen = -2;
 // masked scores: far below any score, and their product with a scale (1e-25 at least) far below
 // any reference, but finite, so that 0 times their distance is 0
 constexpr float kMasked = -1e33f;
@@ -129,15 +132,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                        float scale, __half* __restrict__ out, int64_t ldo, float* __restrict__ H,
                        PagedJoin* __restrict__ joins, float* __restrict__ part) {
   using Cfg = ChunkCfg<D>;
-  constexpr int NS = Cfg::NS, NV = Cfg::NV, T = kChunkTile;
+  constexpr int NS = Cfg::NS, NV = Cfg::NV, NR = Cfg::NR, T = kChunkTile;
+  constexpr bool kWide = TIER == kFP16;
+  constexpr int kHalves = kWide && D == 128 ? 2 : 1;                // rounds of an item (K or V of a tile)
+  constexpr int kUnits = (kWide ? D / 16 : D / 32) / kHalves;       // 16-byte units of a lane per group and round
+  constexpr uint32_t kGroupBytes = kUnits * 512;                    // a group's part of a round
+  static_assert(8 * kGroupBytes <= Cfg::kRawBytes, "a round fits its slot");
   extern __shared__ uint8_t chunk_smem[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chunk_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + 2 * Cfg::kQBytes;
   uint8_t* sV = sK + NS * Cfg::kQBytes;
   uint8_t* sP = sV + NV * Cfg::kVBytes;
-  float4* sMeta = reinterpret_cast<float4*>(sP + 2 * Cfg::kPBytes);  // [kChunkMeta][8 groups]: K factor, V shift, 2^-shift
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sP + 2 * Cfg::kPBytes + Cfg::kMetaBytes);
+  uint8_t* sRaw = sP + 2 * Cfg::kPBytes;
+  // [kChunkMeta][8 groups]: K factor, V shift, 2^-shift, where the group is (its page, or a Where)
+  float4* sMeta = reinterpret_cast<float4*>(sRaw + NR * Cfg::kRawBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(sMeta) + Cfg::kMetaBytes);
   uint64_t* q_full = bars;            // [2] Q tile stored (4 warps)
   uint64_t* k_full = q_full + 2;      // [NS] K tile stored (4 warps)
   uint64_t* k_empty = k_full + NS;    // [NS] both issuers' S MMAs done
@@ -150,12 +160,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* o_free = o_done + 2;      // [2] O_w read out (4 warps)
   uint64_t* drain = o_free + 2;       // [2]
   uint64_t* job_full = drain + 2;     // [2] a job handed out
-  uint64_t* job_empty = job_full + 2; // [2] read by the 14 other warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(job_empty + 2);
+  uint64_t* job_empty = job_full + 2; // [2] read by the 15 other warps
+  uint64_t* raw_full = job_empty + 2; // [NR] a round's copies landed
+  uint64_t* raw_empty = raw_full + NR;  // [NR] read by the key warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + NR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int64_t* s_share = reinterpret_cast<int64_t*>(tmem_slot + 2);
   ChunkJob* jobs = reinterpret_cast<ChunkJob*>(reinterpret_cast<uint8_t*>(bars) + Cfg::kBarBytes - 2 * sizeof(ChunkJob));
-  static_assert((2 + 2 * NS + 2 * NV + 16) * 8 + 8 + 24 + 2 * sizeof(ChunkJob) <= Cfg::kBarBytes, "barrier region overflows");
+  static_assert((2 + 2 * NS + 2 * NV + 16 + 2 * NR) * 8 + 8 + 24 + 2 * sizeof(ChunkJob) <= Cfg::kBarBytes, "barrier region overflows");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -176,7 +188,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&o_free[i], 4);
       mbar_init(&drain[i], 1);
       mbar_init(&job_full[i], 1);
-      mbar_init(&job_empty[i], 14);
+      mbar_init(&job_empty[i], 15);
+    }
+    for (int i = 0; i < NR; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -235,6 +251,82 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         __syncwarp();
       }
       if (!ok) give_up();
+    } else if (warp == 3) {
+      // ------------------------------------------------------------ copies of the keys
+      // Lane l < 8 has group l of every tile: its page, its scales into sMeta, its part of
+      // each round by one bulk copy.  Rounds in the key warps' order: K_0 | K_1 V_0 | K_2 V_1 | ..
+      const int pg = c.page_shift - 4;
+      const float to2 = scale * 1.4426950408889634f;
+      const int64_t part_bytes = c.page_size * D * (kWide ? 2 : 1);  // a page's K or V of a head
+      uint32_t kt = 0, rounds = 0;
+      bool ok = true;
+      while (ok) {
+        ok = next_job();
+        if (!ok || u.nmax < 0) break;
+        const int full = kWide ? INT_MAX : u.length >> c.page_shift;  // blocks in pages
+        const int ends = (u.length + 15) >> 4;                        // groups with tokens
+        const int32_t* table = c.table + u.seq * c.max_pages;
+        auto lookup = [&](int j) -> int {
+          const int g = (u.tile0 + j) * 8 + lane, blk = g >> pg;
+          if (lane >= 8 || j >= u.nmax || g >= ends) return kNowhere;
+          if (blk >= full) return kOpen;
+          const int p = table[blk];
+          return p >= 0 && p < c.num_pages ? p : kNowhere;
+        };
+        auto scales = [&](int p) -> float2 {
+          if (kWide || p < 0) return make_float2(1.f, 1.f);
+          return *reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2);
+        };
+        auto copy = [&](int j, int p, int which) {
+          const uint8_t* src = c.pages + ((static_cast<int64_t>(p) * c.kv_heads + u.h) * 2 + which) * part_bytes +
+                               (((u.tile0 + j) * 8 + lane) & ((1 << pg) - 1)) * (kGroupBytes * kHalves);
+          const unsigned n = __popc(__ballot_sync(0xffffffffu, p >= 0));
+#pragma unroll
+          for (int hh = 0; ok && hh < kHalves; ++hh, ++rounds) {
+            const int slot = rounds % NR;
+            ok = mbar_wait_warp(&raw_empty[slot], ((rounds / NR) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], n * kGroupBytes);
+            __syncwarp();
+            if (p >= 0)
+              bulk_load(sRaw + slot * Cfg::kRawBytes + lane * kGroupBytes, src + hh * kGroupBytes, kGroupBytes, &raw_full[slot]);
+            __syncwarp();
+          }
+        };
+        auto tell = [&](int j, int p, float2 sc) {
+          if (lane >= 8) return;
+          const float lv = v_shift(sc.y, u.log2_vref);
+          float4 m = make_float4(fmaxf(to2 * sc.x, 1e-25f), lv, ex2_approx(-lv), __int_as_float(p));
+          if (p == kNowhere) m = make_float4(1e-25f, kMasked, 1.f, __int_as_float(p));
+          sMeta[((kt + j) % kChunkMeta) * 8 + lane] = m;
+        };
+        int p0 = lookup(0), p1 = lookup(1);  // page numbers a tile ahead of the copies
+        float2 sc = scales(p0);
+        if (u.nmax > 0) {
+          tell(0, p0, sc);
+          __syncwarp();
+          copy(0, p0, 0);
+        }
+        for (int j = 0; ok && j < u.nmax; ++j) {
+          const int p2 = lookup(j + 2);
+          if (j + 1 < u.nmax) {
+            sc = scales(p1);
+            tell(j + 1, p1, sc);
+            __syncwarp();
+            copy(j + 1, p1, 0);
+          }
+          if (ok) copy(j, p0, 1);
+          p0 = p1;
+          p1 = p2;
+        }
+        kt += u.nmax;
+      }
+      if (!ok) {
+        give_up();
+        // the copies in flight land before the CTA can exit (bounded)
+        for (uint32_t i = rounds > NR ? rounds - NR : 0; i < rounds; ++i)
+          (void)mbar_wait(&raw_full[i % NR], (i / NR) & 1u, nullptr);
+      }
     } else if (warp < 2) {
       // ------------------------------------------------------------ UMMA issuers
       constexpr uint32_t idesc_s = make_idesc(1u, 0u, T, T);
@@ -323,9 +415,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // -------------------------------------------------------------- keys
     // Warp kw takes keys 32 kw .. + 31 of every tile: groups 2 kw, 2 kw + 1 of 16.
     const int kw = warp - 4, gq = lane >> 2, q4 = lane & 3;
-    const float to2 = scale * 1.4426950408889634f;
     const int pg = c.page_shift - 4;
-    uint32_t kt = 0, vt = 0;
+    uint32_t kt = 0, vt = 0, rounds = 0;
     bool ok = true;
     // K row of group ga, half hf: 16 (2 kw + ga) + 8 hf + gq, so row & 7 = gq
     auto k_at = [&](uint8_t* tile, int ga, int hf, int piece, int cc) -> uint4* {
@@ -335,198 +426,165 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     auto v_at = [&](uint8_t* tile, int i) -> uint4* {  // dimension gq D/8 + i
       return reinterpret_cast<uint4*>(tile + (kw >> 1) * (D * 128) + (8 * i + gq) * 128 + (((2 * q4 + (kw & 1)) ^ gq) << 4));
     };
-    // x: eight or fewer 16-byte units of each of the two groups.  An item (K or V of a tile) takes
-    // kHalves rounds of x; a unit is refilled for the next round as soon as it is used.
-    constexpr bool kWide = TIER == kFP16;
-    constexpr int kHalves = kWide && D == 128 ? 2 : 1;
-    constexpr int kUnits = (kWide ? D / 16 : D / 32) / kHalves;  // per group and round
     constexpr int kCodes = kWide ? kINT8 : TIER;
     uint4 x[2][kUnits];
+    // the next round into registers; its slot is free again
+    auto take = [&]() {
+      const int slot = rounds % NR;
+      ok = mbar_wait_warp(&raw_full[slot], (rounds / NR) & 1u, abort_flag);
+      if (!ok) return;
+      const uint4* src = reinterpret_cast<const uint4*>(sRaw + slot * Cfg::kRawBytes + 2 * kw * kGroupBytes) + lane;
+#pragma unroll
+      for (int ga = 0; ga < 2; ++ga)
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) x[ga][i] = src[ga * (kGroupBytes / 16) + 32 * i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[slot]);
+      ++rounds;
+    };
     while (ok) {
       ok = next_job();
       if (!ok || u.nmax < 0) break;
-      if (u.nmax == 0) continue;
-      const int full = kWide ? INT_MAX : u.length >> c.page_shift;  // blocks in pages
-      const int ends = (u.length + 15) >> 4;                        // groups with tokens
-      const int32_t* table = c.table + u.seq * c.max_pages;
-      const float log2_vref = u.log2_vref;
+      const int full = u.length >> c.page_shift;
       const int gbase = u.tile0 * 8 + 2 * kw;  // this warp's first group of tile 0 of the part
-      // where a group's values are: nowhere (-1: a hole, or past the tokens), page p, the open block
-      struct Pages {
-        int p[2];
-      };
-      auto lookup = [&](int j) -> Pages {
-        Pages r;
-#pragma unroll
-        for (int ga = 0; ga < 2; ++ga) {
-          const int g = gbase + 8 * j + ga, blk = g >> pg;
-          int p = -1;
-          if (j < u.nmax && g < ends) {
-            if (blk >= full) {
-              p = INT_MAX;
-            } else {
-              p = __ldg(table + blk);
-              p = p >= 0 && p < c.num_pages ? p : -1;
-            }
-          }
-          r.p[ga] = p;
-        }
-        return r;
-      };
-      // a group's first unit of this lane (K: which 0, V: 1), null where nothing is prefetched
-      auto source = [&](const Pages& r, int j, int which, int ga) -> const uint4* {
-        const int g = (gbase + 8 * j + ga) & ((1 << pg) - 1);
-        if (r.p[ga] < 0 || r.p[ga] == INT_MAX) return nullptr;
-        return reinterpret_cast<const uint4*>(paged_block(c, r.p[ga], u.h, which)) + g * (kWide ? 2 * D : D) + lane;
-      };
+      // the open block's fp16 rows, which the copies leave out
       auto open_source = [&](int j, int which, int ga) -> const uint4* {
         const int g = (gbase + 8 * j + ga) & ((1 << pg) - 1);
         return reinterpret_cast<const uint4*>(paged_open(c, u.seq, full, u.h, which)) + g * 2 * D + lane;
       };
-      auto fetch = [](const uint4* src, int i) -> uint4 { return src ? __ldg(src + 32 * i) : make_uint4(0, 0, 0, 0); };
-      auto scales = [&](const Pages& r) -> float2 {  // lanes 0, 1: of their group
-        const int p = lane == 0 ? r.p[0] : r.p[1];
-        if (kWide || lane > 1 || p < 0 || p == INT_MAX) return make_float2(1.f, 1.f);
-        return __ldg(reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2));
+      auto nothing = [](uint4 (&v)[kUnits]) {  // what stands for zeros
+        const uint32_t z = kWide || TIER != kINT8 ? 0u : 0x80808080u;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) v[i] = make_uint4(z, z, z, z);
       };
-      auto zero_code = [](uint4 v, bool there) -> uint4 {  // a hole's codes stand for zeros
-        if (kWide || TIER != kINT8 || there) return v;
-        return make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-      };
-
-      // the item after the one in x: its sources
-      const uint4* nsrc[2];
-      auto aim = [&](const Pages& r, int j, int which) {
-        nsrc[0] = source(r, j, which, 0);
-        nsrc[1] = source(r, j, which, 1);
-      };
-      auto k_item = [&](const Pages& r, int j, float2 sc) {  // stores K of tile j from x, refills x from nsrc
-        const uint32_t idx = kt + j;
-        const int stage = idx % NS;
-        ok = mbar_wait_warp(&k_empty[stage], ((idx / NS) & 1u) ^ 1u, abort_flag);
-        if (!ok) return;
-        uint8_t* dst = sK + stage * Cfg::kQBytes;
-        if (lane < 2) {
-          const int p = lane == 0 ? r.p[0] : r.p[1];
-          const float lv = v_shift(sc.y, log2_vref);
-          sMeta[(idx % kChunkMeta) * 8 + 2 * kw + lane] =
-              p < 0 ? make_float4(1e-25f, kMasked, 1.f, 0.f) : make_float4(fmaxf(to2 * sc.x, 1e-25f), lv, ex2_approx(-lv), 0.f);
-        }
-        const uint4* own[2] = {source(r, j, 0, 0), source(r, j, 0, 1)};
+      for (int j = -1; ok && j < u.nmax; ++j) {
+        if (j + 1 < u.nmax) {  // K of tile j + 1
+          const uint32_t idx = kt + j + 1;
+          const int stage = idx % NS;
+          uint8_t* dst = sK + stage * Cfg::kQBytes;
 #pragma unroll
-        for (int hh = 0; hh < kHalves; ++hh) {
-#pragma unroll
-          for (int ga = 0; ga < 2; ++ga) {
-            const uint4* refill = hh + 1 < kHalves ? own[ga] : nsrc[ga];
-            if (!kWide && r.p[ga] == INT_MAX) {  // the open block's fp16 rows
-              const uint4* src = open_source(j, 0, ga);
-#pragma unroll
-              for (int i = 0; i < D / 16; ++i) *k_at(dst, ga, i / (D / 32), (i % (D / 32)) >> 1, i & 1) = __ldg(src + 32 * i);
-#pragma unroll
-              for (int i = 0; i < kUnits; ++i) x[ga][i] = fetch(refill, i);
-            } else {
-#pragma unroll
-              for (int i = 0; i < kUnits; ++i) {
-                if constexpr (kWide) {
-                  const int k = hh * kUnits + i;
-                  *k_at(dst, ga, k / (D / 32), (k % (D / 32)) >> 1, k & 1) = x[ga][i];
-                } else {
-                  const uint4 v = zero_code(x[ga][i], r.p[ga] >= 0);
-                  uint4 a, b;
-                  codes_to_h2<kCodes>(v.x, a.x, a.y);
-                  codes_to_h2<kCodes>(v.y, a.z, a.w);
-                  codes_to_h2<kCodes>(v.z, b.x, b.y);
-                  codes_to_h2<kCodes>(v.w, b.z, b.w);
-                  *k_at(dst, ga, i / (D / 64), i % (D / 64), 0) = a;
-                  *k_at(dst, ga, i / (D / 64), i % (D / 64), 1) = b;
-                }
-                x[ga][i] = fetch(refill, (hh + 1 < kHalves ? (hh + 1) * kUnits : 0) + i);
-              }
-            }
-          }
-        }
-        fence_proxy_async_shared();  // the stores, visible to the tensor core
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&k_full[stage]);
-      };
-      auto v_item = [&](const Pages& r, int j) {
-        const uint32_t idx = vt + j;
-        const int stage = idx % NV;
-        ok = mbar_wait_warp(&v_empty[stage], ((idx / NV) & 1u) ^ 1u, abort_flag);
-        if (!ok) return;
-        uint8_t* dst = sV + stage * Cfg::kVBytes;
-        const bool open0 = !kWide && r.p[0] == INT_MAX, open1 = !kWide && r.p[1] == INT_MAX;
-        const uint4* own[2] = {source(r, j, 1, 0), source(r, j, 1, 1)};
-        uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};  // tokens past the sequence's are no numbers to multiply by
-        if (kWide || open0 || open1) {
-#pragma unroll
-          for (int ga = 0; ga < 2; ++ga)
-#pragma unroll
-            for (int th = 0; th < 2; ++th) {
-              const int t0 = (gbase + 8 * j + ga) * 16 + 2 * q4 + 8 * th;
-              keep[ga][th] = (t0 < u.length ? 0xffffu : 0u) | (t0 + 1 < u.length ? 0xffff0000u : 0u);
-            }
-        }
-        const uint4* os[2] = {open0 ? open_source(j, 1, 0) : nullptr, open1 ? open_source(j, 1, 1) : nullptr};
-#pragma unroll
-        for (int hh = 0; hh < kHalves; ++hh) {
-#pragma unroll
-          for (int m = 0; m < D / 16 / kHalves; ++m) {
-            const int mb = hh * (D / 16 / kHalves) + m, i = kWide ? m : m >> 1;
-            uint32_t j0[4], j1[4];  // dimensions 2 mb, 2 mb + 1: two pairs of keys of group 0, of group 1
+          for (int hh = 0; hh < kHalves; ++hh) {
+            take();
+            if (ok && hh == 0) ok = mbar_wait_warp(&k_empty[stage], ((idx / NS) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
+            const float4* meta = sMeta + (idx % kChunkMeta) * 8 + 2 * kw;
 #pragma unroll
             for (int ga = 0; ga < 2; ++ga) {
-              if (kWide || (ga ? open1 : open0)) {
-                const uint4 y = kWide ? x[ga][i] : __ldg(os[ga] + 32 * mb);
-                j0[2 * ga] = y.x & keep[ga][0];
-                j1[2 * ga] = y.y & keep[ga][0];
-                j0[2 * ga + 1] = y.z & keep[ga][1];
-                j1[2 * ga + 1] = y.w & keep[ga][1];
+              const int where = __float_as_int(meta[ga].w);
+              if (where == kNowhere) nothing(x[ga]);
+              if (!kWide && where == kOpen) {
+                const uint4* src = open_source(j + 1, 0, ga);
+                uint4 y[D / 16];
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) y[i] = __ldg(src + 32 * i);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) *k_at(dst, ga, i / (D / 32), (i % (D / 32)) >> 1, i & 1) = y[i];
               } else {
-                const uint4 v = zero_code(x[ga][i], r.p[ga] >= 0);
-                codes_to_h2<kCodes>(m & 1 ? v.z : v.x, j0[2 * ga], j1[2 * ga]);
-                codes_to_h2<kCodes>(m & 1 ? v.w : v.y, j0[2 * ga + 1], j1[2 * ga + 1]);
+#pragma unroll
+                for (int i = 0; i < kUnits; ++i) {
+                  if constexpr (kWide) {
+                    const int k = hh * kUnits + i;
+                    *k_at(dst, ga, k / (D / 32), (k % (D / 32)) >> 1, k & 1) = x[ga][i];
+                  } else {
+                    uint4 a, b;
+                    codes_to_h2<kCodes>(x[ga][i].x, a.x, a.y);
+                    codes_to_h2<kCodes>(x[ga][i].y, a.z, a.w);
+                    codes_to_h2<kCodes>(x[ga][i].z, b.x, b.y);
+                    codes_to_h2<kCodes>(x[ga][i].w, b.z, b.w);
+                    *k_at(dst, ga, i / (D / 64), i % (D / 64), 0) = a;
+                    *k_at(dst, ga, i / (D / 64), i % (D / 64), 1) = b;
+                  }
+                }
               }
             }
-            *v_at(dst, 2 * mb) = make_uint4(j0[0], j0[1], j0[2], j0[3]);
-            *v_at(dst, 2 * mb + 1) = make_uint4(j1[0], j1[1], j1[2], j1[3]);
-            if (kWide || (m & 1)) {
+          }
+          if (!ok) break;
+          fence_proxy_async_shared();  // the stores, visible to the tensor core
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&k_full[stage]);
+        }
+        if (j >= 0) {  // V of tile j
+          const uint32_t idx = vt + j;
+          const int stage = idx % NV;
+          uint8_t* dst = sV + stage * Cfg::kVBytes;
 #pragma unroll
-              for (int ga = 0; ga < 2; ++ga)
-                x[ga][i] = fetch(hh + 1 < kHalves ? own[ga] : nsrc[ga], (hh + 1 < kHalves ? (hh + 1) * kUnits : 0) + i);
+          for (int hh = 0; hh < kHalves; ++hh) {
+            take();
+            if (ok && hh == 0) ok = mbar_wait_warp(&v_empty[stage], ((idx / NV) & 1u) ^ 1u, abort_flag);
+            if (!ok) break;
+            const float4* meta = sMeta + (idx % kChunkMeta) * 8 + 2 * kw;
+            const int w0 = __float_as_int(meta[0].w), w1 = __float_as_int(meta[1].w);
+            const bool open0 = !kWide && w0 == kOpen, open1 = !kWide && w1 == kOpen;
+            if (w0 == kNowhere) nothing(x[0]);
+            if (w1 == kNowhere) nothing(x[1]);
+            // tokens past the sequence's are no numbers to multiply by (only fp16 rows can be)
+            uint32_t keep[2][2];
+#pragma unroll
+            for (int ga = 0; ga < 2; ++ga)
+#pragma unroll
+              for (int th = 0; th < 2; ++th) {
+                const int t0 = (gbase + 8 * j + ga) * 16 + 2 * q4 + 8 * th;
+                keep[ga][th] = (t0 < u.length ? 0xffffu : 0u) | (t0 + 1 < u.length ? 0xffff0000u : 0u);
+              }
+            auto put = [&](int mb, const uint32_t (&j0)[4], const uint32_t (&j1)[4]) {
+              *v_at(dst, 2 * mb) = make_uint4(j0[0], j0[1], j0[2], j0[3]);
+              *v_at(dst, 2 * mb + 1) = make_uint4(j1[0], j1[1], j1[2], j1[3]);
+            };
+            auto wide = [&](const uint4& y, int ga, uint32_t (&j0)[4], uint32_t (&j1)[4]) {
+              j0[2 * ga] = y.x & keep[ga][0];
+              j1[2 * ga] = y.y & keep[ga][0];
+              j0[2 * ga + 1] = y.z & keep[ga][1];
+              j1[2 * ga + 1] = y.w & keep[ga][1];
+            };
+            auto code = [&](int m, int ga, uint32_t (&j0)[4], uint32_t (&j1)[4]) {
+              const uint4 v = x[ga][kWide ? 0 : m >> 1];
+              codes_to_h2<kCodes>(m & 1 ? v.z : v.x, j0[2 * ga], j1[2 * ga]);
+              codes_to_h2<kCodes>(m & 1 ? v.w : v.y, j0[2 * ga + 1], j1[2 * ga + 1]);
+            };
+            if (kWide) {
+#pragma unroll
+              for (int m = 0; m < kUnits; ++m) {
+                uint32_t j0[4], j1[4];
+                wide(x[0][m], 0, j0, j1);
+                wide(x[1][m], 1, j0, j1);
+                put(hh * kUnits + m, j0, j1);
+              }
+            } else if (!open0 && !open1) {
+#pragma unroll
+              for (int m = 0; m < D / 16; ++m) {
+                uint32_t j0[4], j1[4];
+                code(m, 0, j0, j1);
+                code(m, 1, j0, j1);
+                put(m, j0, j1);
+              }
+            } else {
+              const uint4* os0 = open_source(j, 1, 0);
+              const uint4* os1 = open_source(j, 1, 1);
+#pragma unroll
+              for (int mq = 0; mq < D / 16; mq += 4) {
+                uint4 y0[4], y1[4];
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  y0[m] = open0 ? __ldg(os0 + 32 * (mq + m)) : make_uint4(0, 0, 0, 0);
+                  y1[m] = open1 ? __ldg(os1 + 32 * (mq + m)) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  uint32_t j0[4], j1[4];
+                  if (open0) wide(y0[m], 0, j0, j1);
+                  else code(mq + m, 0, j0, j1);
+                  if (open1) wide(y1[m], 1, j0, j1);
+                  else code(mq + m, 1, j0, j1);
+                  put(mq + m, j0, j1);
+                }
+              }
             }
           }
-        }
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[stage]);
-      };
-
-      // K_0 | K_1 V_0 | K_2 V_1 | ..; page numbers a tile ahead of the loads that need them
-      Pages p0 = lookup(0), p1 = lookup(1);
-      float2 sc = scales(p0);
-      aim(p0, 0, 0);
-#pragma unroll
-      for (int ga = 0; ga < 2; ++ga)
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) x[ga][i] = fetch(nsrc[ga], i);
-      float2 sc1 = scales(p1);
-      if (u.nmax > 1) aim(p1, 1, 0);
-      else aim(p0, 0, 1);
-      k_item(p0, 0, sc);
-      for (int j = 0; ok && j < u.nmax; ++j) {  // x: K of tile j + 1, or V of tile j if it is the last
-        const Pages p2 = lookup(j + 2);
-        if (j + 1 < u.nmax) {
-          aim(p0, j, 1);
-          k_item(p1, j + 1, sc1);
           if (!ok) break;
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[stage]);
         }
-        sc1 = scales(p2);
-        if (j + 2 < u.nmax) aim(p2, j + 2, 0);
-        else aim(p1, j + 1, 1);  // past the last tile: p1 holds nothing, and nothing is loaded
-        v_item(p0, j);
-        p0 = p1;
-        p1 = p2;
       }
       kt += u.nmax;
       vt += u.nmax;
