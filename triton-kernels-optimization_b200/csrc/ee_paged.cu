@@ -67,14 +67,21 @@ int run_read(const PagedArgs& c, const PagedStepArgs& st, __half* k, int64_t ldk
                     paged_stage_bytes(static_cast<int>(c.page_size), D), s, c, st, k, ldk, v, ldv);
 }
 
-// CTAs per SM of the few-row kernel, by its launch bounds
-constexpr int few_ctas(int nb) { return nb == 1 ? 3 : 2; }
-
-template <int D, int TIER, int NB>
+// CTAs of the few-row kernel: as many as are resident; each has a ticket, and a weight in the
+// kernel's shared memory
+constexpr int kFewMaxCtas = 1024;
+template <int D, int TIER, int NB, int RS>
 int run_few(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, const PagedRows& q, int heads, float scale,
             __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
-  return launch_pdl(paged_attention_kernel<D, TIER, NB>, dim3(static_cast<unsigned>(sm_count() * few_ctas(NB))),
-                    dim3(kFewThreads), 0, s, c, st, pl, q, heads, scale, out, ldo, H, tickets, part);
+  using Cfg = FewCfg<D, TIER, NB, RS>;
+  int e = allow_smem<paged_attention_kernel<D, TIER, NB, RS>>(Cfg::kSmem);
+  if (e != 0) return e;
+  static_assert(Cfg::kSmem <= 227 * 1024, "few-row attention above the 227 KB of shared memory per CTA");
+  constexpr int per_smem = static_cast<int>(227 * 1024 / (Cfg::kSmem + 1024));
+  constexpr int per = Cfg::kCtas < per_smem ? Cfg::kCtas : per_smem;
+  const int n = std::min(sm_count() * per, std::min(kFewMaxCtas, Cfg::kRowRoom));
+  return launch_pdl(paged_attention_kernel<D, TIER, NB, RS>, dim3(static_cast<unsigned>(n)), dim3(Cfg::kThreads), Cfg::kSmem, s,
+                    c, st, pl, q, heads, scale, out, ldo, H, tickets, part);
 }
 template <int D, int TIER>
 int run_chunk(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, const PagedRows& q, int heads, float scale,
@@ -87,28 +94,28 @@ int run_chunk(const PagedArgs& c, const PagedStepArgs& st, const PagedPlan& pl, 
   e = launch_pdl(paged_chunk_kernel<D, TIER>, dim3(n), dim3(kChunkThreads), ChunkCfg<D>::kSmem, s, c, st, pl, q, heads,
                  scale, out, ldo, H, joins, part);
   if (e != 0) return e;
-  return launch_pdl(paged_join_kernel<D>, dim3(n, 8), dim3(256), 0, s, pl, static_cast<const PagedJoin*>(joins), heads, out,
+  return launch_pdl(paged_join_kernel<D>, dim3(n, 8, D / 32), dim3(256), 0, s, pl, static_cast<const PagedJoin*>(joins), heads, out,
                     ldo, H, static_cast<const float*>(part));
 }
 template <int D, int TIER>
 int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& q, int heads, int64_t max_new, float scale,
                   __half* out, int64_t ldo, float* H, uint32_t* tickets, float* part, cudaStream_t s) {
   const int G = heads / static_cast<int>(c.kv_heads);
-  // query rows of one KV head that a unit holds: 8 or 16 (mma.sync, bound by the cache's
+  // query rows of one KV head that a unit holds: 8, 16 or 32 (mma.sync, bound by the cache's
   // bytes), or two tiles of 128 (tcgen05)
   const int64_t rows = G * max_new;
-  const int R = rows <= 8 ? 8 : (rows <= 16 ? 16 : 128);
+  const int R = rows <= 8 ? 8 : (rows <= 16 ? 16 : (rows <= 32 ? 32 : 128));
   PagedPlan pl;
   pl.G = G;
   pl.hgroups = (G + R - 1) / R;
   pl.Gc = (G + pl.hgroups - 1) / pl.hgroups;
   pl.TQ = R / pl.Gc;
-  pl.fixed = 64;
-  // no CTA for less than four turns of its warps: shorter parts cost more in joining than
-  // they save
+  pl.fixed = 2 * kFewTile;
+  // no CTA for less than four stages: shorter parts cost more in joining than they save
   pl.min_cost = 4 * kFewTile;
-  if (R == 8) return run_few<D, TIER, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
-  if (R == 16) return run_few<D, TIER, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  if (R == 8) return run_few<D, TIER, 1, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  if (R == 16) return run_few<D, TIER, 2, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
+  if (R == 32) return run_few<D, TIER, 2, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
   pl.TQ *= 2;
   pl.fixed = 2 * kChunkTile;
   pl.min_cost = 4 * kChunkTile;
@@ -119,7 +126,7 @@ int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& 
 size_t paged_head_bytes() { return 4096; }  // a ticket per CTA
 size_t paged_workspace_bytes(int64_t D) {
   // two parts per CTA: 16 rows of the few-row kernel's CTAs, 256 of the chunk kernel's
-  return paged_head_bytes() + size_t(2) * sm_count() * std::max<size_t>(few_ctas(1) * 16 * (D + 4), 256 * (D + 3)) * sizeof(float) +
+  return paged_head_bytes() + size_t(2) * sm_count() * std::max<size_t>(3 * 32 * (D + 4), 256 * (D + 3)) * sizeof(float) +
          kChunkJoinBytes;
 }
 

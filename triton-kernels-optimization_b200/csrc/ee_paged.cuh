@@ -723,21 +723,21 @@ __device__ __forceinline__ float v_shift(float vs, float log2_vref) {
   return vs < __builtin_huge_valf() ? x : __builtin_nanf("");
 }
 
-constexpr int kFewWarps = 4;
-constexpr int kFewThreads = 32 * kFewWarps;
-constexpr int kFewTile = 16 * kFewWarps;  // keys per turn of the CTA
 constexpr float kNegInf = -__builtin_huge_valf();
+// where a group of 16 keys is, besides page p >= 0: nowhere (a hole, or past the tokens), in the open block
+constexpr int kNowhere = -1, kOpen = -2;
 
-// NB blocks of eight rows (rows = query heads of the unit x its tokens) per unit.  Warp w takes
-// every kFewWarps-th group of 16 keys.  Scores S^T = K Q^T (keys are the MMA's rows, so that
-// eight query rows fill its columns), each lane holding rows 2 q4, 2 q4 + 1 of keys gq, gq + 8;
-// the online softmax per row with a reference that moves only when a score outgrows it by
-// 2^8; P^T, transposed in registers, as the B operand of O^T += V^T P^T, whose columns are the
-// same two rows in every lane.  The next group's codes are loaded before this one is used.
+constexpr int kFewGroups = 4;               // groups of 16 keys per ring stage
+constexpr int kFewTile = 16 * kFewGroups;   // keys per stage
+
+// NB blocks of eight rows (rows = query heads of the unit x its tokens) per warp.  Scores
+// S^T = K Q^T of 16 keys (keys are the MMA's rows, so that eight query rows fill its columns),
+// each lane holding rows 2 q4, 2 q4 + 1 of keys gq, gq + 8; the online softmax per row with a
+// reference that moves only when a score outgrows it by 2^8; P^T, transposed in registers, as
+// the B operand of O^T += V^T P^T, whose columns are the same two rows in every lane.
 template <int D, int TIER, int NB>
 struct FewRows {
   static constexpr int KB = D / 16;
-  static constexpr int R = 8 * NB;
   uint32_t q[NB][2 * KB];
   float o[NB][KB][4];
   float m[NB][2], l[NB][2], t[NB][2];
@@ -753,8 +753,8 @@ struct FewRows {
   }
   // s: scores of 16 keys from key0; f the factor to base-2 logits, lv / inv the V shift and
   // 2^-lv; lim: keys that rows 2 q4 (+ 1) of each block see; pb: P^T's B operand
-  __device__ __forceinline__ void softmax(float (&s)[NB][4], float f, float lv, float inv, int64_t key0, bool edge,
-                                          const int64_t (&lim)[NB][2], int gq, uint32_t (&pb)[NB][2]) {
+  __device__ __forceinline__ void softmax(float (&s)[NB][4], float f, float lv, float inv, int key0, bool edge,
+                                          const int (&lim)[NB][2], int gq, uint32_t (&pb)[NB][2]) {
     bool grow = false;
     float y[NB][4];
 #pragma unroll
@@ -811,114 +811,300 @@ struct FewRows {
       pb[n][1] = transpose8(pack2(p[2], p[3]));
     }
   }
-  // 16 keys held in 8 bits
-  __device__ __forceinline__ void codes(const uint4 (&kq)[D / 32], const uint4 (&vq)[D / 32], float f, float lv, float inv,
-                                        int64_t key0, bool edge, const int64_t (&lim)[NB][2], int gq) {
-    float s[NB][4];
+  // 16 keys in 8 bits; kp / vp: this lane's first unit; taken(): the values are in registers
+  template <typename F>
+  __device__ __forceinline__ void codes(const uint4* kp, const uint4* vp, float f, float lv, float inv, int key0, bool edge,
+                                        const int (&lim)[NB][2], int gq, F taken) {
+    constexpr int TC = TIER == kFP16 ? kINT8 : TIER;
+    uint4 u[D / 32];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(kq);  // [half][KB] words
+    for (int i = 0; i < D / 32; ++i) u[i] = kp[i * 32];
+    float s[NB][4], s2[NB][4];  // two chains: one MMA waits for the last but one
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);  // [half][KB] words
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
       uint32_t a[4];
-      codes_to_h2<TIER>(kw[kb], a[0], a[2]);
-      codes_to_h2<TIER>(kw[KB + kb], a[1], a[3]);
+      codes_to_h2<TC>(w[kb], a[0], a[2]);
+      codes_to_h2<TC>(w[KB + kb], a[1], a[3]);
 #pragma unroll
-      for (int n = 0; n < NB; ++n) mma_16816(s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
+      for (int n = 0; n < NB; ++n) mma_16816(kb & 1 ? s2[n] : s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
     }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) u[i] = vp[i * 32];  // [mb][th] words
+    taken();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
     uint32_t pb[NB][2];
     softmax(s, f, lv, inv, key0, edge, lim, gq, pb);
-    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vq);  // [mb][th] words
 #pragma unroll
     for (int mb = 0; mb < KB; ++mb) {
       uint32_t a[4];
-      codes_to_h2<TIER>(vw[2 * mb], a[0], a[1]);
-      codes_to_h2<TIER>(vw[2 * mb + 1], a[2], a[3]);
+      codes_to_h2<TC>(w[2 * mb], a[0], a[1]);
+      codes_to_h2<TC>(w[2 * mb + 1], a[2], a[3]);
 #pragma unroll
       for (int n = 0; n < NB; ++n) mma_16816(o[n][mb], a, pb[n][0], pb[n][1]);
     }
   }
-  // 16 keys held in fp16 (kp / vp: this lane's first unit); tokens from `length` on are not there
-  __device__ __forceinline__ void wide(const uint4* kp, const uint4* vp, float f, float lv, float inv, int64_t key0, bool edge,
-                                       int64_t length, const int64_t (&lim)[NB][2], int gq, int q4) {
-    uint4 ku[D / 16], vu[D / 16];
+  // 16 keys in fp16; tokens from `length` on are not there
+  template <typename F>
+  __device__ __forceinline__ void wide(const uint4* kp, const uint4* vp, float f, float lv, float inv, int key0, bool edge,
+                                       int length, const int (&lim)[NB][2], int gq, int q4, F taken) {
+    uint4 u[D / 16];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) ku[i] = kp[i * 32];
+    for (int i = 0; i < D / 16; ++i) u[i] = kp[i * 32];
+    float s[NB][4], s2[NB][4];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) vu[i] = vp[i * 32];
-    float s[NB][4];
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    const uint32_t* kw = reinterpret_cast<const uint32_t*>(ku);  // [half][KB][2] words
+      for (int i = 0; i < 4; ++i) s[n][i] = s2[n][i] = 0.f;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(u);  // [half][KB][2] words
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const uint32_t a[4] = {kw[2 * kb], kw[2 * KB + 2 * kb], kw[2 * kb + 1], kw[2 * KB + 2 * kb + 1]};
+      const uint32_t a[4] = {w[2 * kb], w[2 * KB + 2 * kb], w[2 * kb + 1], w[2 * KB + 2 * kb + 1]};
 #pragma unroll
-      for (int n = 0; n < NB; ++n) mma_16816(s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
+      for (int n = 0; n < NB; ++n) mma_16816(kb & 1 ? s2[n] : s[n], a, q[n][2 * kb], q[n][2 * kb + 1]);
     }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) u[i] = vp[i * 32];
+    taken();
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] += s2[n][i];
     uint32_t pb[NB][2];
     softmax(s, f, lv, inv, key0, edge, lim, gq, pb);
     uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
     if (key0 + 16 > length) {  // what lies past the sequence's tokens is no number to multiply by
 #pragma unroll
       for (int th = 0; th < 2; ++th) {
-        const int64_t t0 = key0 + 2 * q4 + 8 * th;
+        const int t0 = key0 + 2 * q4 + 8 * th;
         keep[th] = (t0 < length ? 0xffffu : 0u) | (t0 + 1 < length ? 0xffff0000u : 0u);
       }
     }
-    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vu);
 #pragma unroll
     for (int mb = 0; mb < KB; ++mb) {
-      const uint32_t a[4] = {vw[4 * mb] & keep[0], vw[4 * mb + 1] & keep[0], vw[4 * mb + 2] & keep[1],
-                             vw[4 * mb + 3] & keep[1]};
+      const uint32_t a[4] = {w[4 * mb] & keep[0], w[4 * mb + 1] & keep[0], w[4 * mb + 2] & keep[1], w[4 * mb + 3] & keep[1]};
 #pragma unroll
       for (int n = 0; n < NB; ++n) mma_16816(o[n][mb], a, pb[n][0], pb[n][1]);
     }
   }
 };
 
-template <int D, int TIER, int NB>
-__global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
+// A part as the copying warp hands it to the others.
+struct __align__(16) FewJob {
+  int tile0, tile1, groups, length;  // stages; groups that the unit's rows reach; tokens (tile1 < 0: no more)
+  int seq, h, hg, pos;               // pos: position of the unit's first token
+  int ntok, row, whole, first;       // tokens; its query row
+  int cta0, cta1;
+  float vref, pad;
+};
+
+template <int D, int TIER, int NB, int RS>
+struct FewCfg {
+  static constexpr bool kWide = TIER == kFP16;
+  static constexpr int R = 8 * NB * RS;                        // rows per unit: RS sets of warps, each with all keys
+  static constexpr int kWarps = kFewGroups * RS;               // the sets' warps
+  static constexpr int kThreads = 32 * (kWarps + 1);           // and the copying one
+  static constexpr int kGroupBytes = 16 * D * (kWide ? 2 : 1); // K, or V
+  static constexpr int kStageBytes = 2 * kFewGroups * kGroupBytes;
+  static constexpr int NS = kStageBytes > 24 * 1024 ? 2 : 48 * 1024 / kStageBytes;
+  static constexpr int kOutRow = D + 4;
+  static constexpr int kCtas = NB == 1 ? 3 : (RS == 1 ? 2 : 1);  // per SM, by the launch bounds
+  static constexpr int kRowRoom = kFewGroups * kOutRow > kCtas * 160 ? kFewGroups * kOutRow : kCtas * 160;
+  static constexpr int kOutBytes = R * kRowRoom * 4;  // the groups' rows, then a weight per part
+  static constexpr int kRec = D + 4;  // a part's row: m, l, t, -, O
+  // ring, rows of the warps, (m, l, t) of the warps, metadata, jobs, barriers
+  static constexpr size_t kSmem = 128 + size_t(NS) * kStageBytes + kOutBytes + kFewGroups * R * 16 + NS * kFewGroups * 16 +
+                                  2 * sizeof(FewJob) + (2 * NS + 5) * 8 + 64;
+};
+
+// CTAs of kWarps + 1 warps, two or three per SM.  The copying warp walks the CTA's share of the
+// line, a part ahead of the others, and keeps the ring full: per stage 4 groups of 16 keys, a
+// bulk copy each for a group's K and V (lane l looks up group l % 4 of stage l / 4, eight stages
+// at a time), with the group's scales.  Warp (set, g) takes group g of every stage.  At the end
+// of a part the warps' rows are joined, and a unit's last CTA joins its parts.
+// Bound by the cache's bytes: HBM's share of an SM is about 23 bytes a cycle, 11 cycles for the
+// K and V codes of a token (D 128); converting them (two ALU operations per fp16 pair) and the
+// MMAs take about 4.
+// The open block's fp16 rows do not fit a stage of codes: the warps read them themselves.
+template <int D, int TIER, int NB, int RS>
+__global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, TIER, NB, RS>::kCtas)
     paged_attention_kernel(const PagedArgs c, const PagedStepArgs st, const PagedPlan pl, const PagedRows q, int heads,
                            float scale, __half* __restrict__ out, int64_t ldo, float* __restrict__ H,
                            uint32_t* __restrict__ tickets, float* __restrict__ part) {
-  constexpr int R = 8 * NB, KB = D / 16, REC = D + 4;  // record of a row: m, l, t, -, O
-  __shared__ float s_o[kFewWarps][R][D + 4];
-  __shared__ float s_st[kFewWarps][R][3];
-  __shared__ int64_t s_share[3];
-  __shared__ uint32_t s_last;
+  using Cfg = FewCfg<D, TIER, NB, RS>;
+  constexpr int R = Cfg::R, KB = D / 16, REC = Cfg::kRec, NS = Cfg::NS, NT = 32 * Cfg::kWarps;
+  constexpr bool kWide = Cfg::kWide;
+  extern __shared__ __align__(128) uint8_t few_smem[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(few_smem) + 127) & ~uintptr_t(127));
+  float* s_o = reinterpret_cast<float*>(ring + NS * Cfg::kStageBytes);           // [group][R][D + 4]
+  float4* s_st = reinterpret_cast<float4*>(s_o + R * Cfg::kRowRoom);  // [group][R]
+  float4* s_meta = s_st + kFewGroups * R;                                        // [NS][group]
+  FewJob* jobs = reinterpret_cast<FewJob*>(s_meta + NS * kFewGroups);
+  uint64_t* full = reinterpret_cast<uint64_t*>(jobs + 2);
+  uint64_t* empty = full + NS;
+  uint64_t* job_full = empty + NS;
+  uint64_t* job_empty = job_full + 2;
+  uint64_t* meet = job_empty + 2;
+  int64_t* s_share = reinterpret_cast<int64_t*>(meet + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 3);
+  volatile uint32_t* s_last = reinterpret_cast<volatile uint32_t*>(s_share + 3) + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, q4 = lane & 3;
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], Cfg::kWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&job_full[i], 1);
+      mbar_init(&job_empty[i], Cfg::kWarps);
+    }
+    mbar_init(meet, Cfg::kWarps);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
   griddep_wait();
   PagedWalk walk = paged_begin(c, st, pl, blockIdx.x, gridDim.x, s_share);
+  if (walk.left <= 0) return;
   const float to2 = scale * 1.4426950408889634f;
+  const int pg = c.page_shift - 4;  // groups per page, log2
+  bool ok = true;
 
+  if (warp == Cfg::kWarps) {
+    // -------------------------------------------------------------- copies
+    const int64_t part_bytes = c.page_size * D * (kWide ? 2 : 1);  // a page's K or V of a head
+    uint32_t stages = 0;
+    PagedPart u;
+    bool more = true;
+    for (uint32_t k = 0; ok && more; ++k) {
+      more = paged_next<kFewTile>(c, st, pl, walk, u);
+      FewJob job = {};
+      job.tile1 = -1;
+      const int fullb = kWide ? c.max_pages : static_cast<int>(u.s.length >> c.page_shift);  // blocks in pages
+      const int groups = static_cast<int>((u.reach + 15) >> 4);
+      const int32_t* table = c.table + u.s.seq * c.max_pages;
+      // eight stages' groups, one per lane: their pages, their scales
+      auto lookup = [&](int chunk) -> int {
+        const int g = (u.tile0 + 8 * chunk) * kFewGroups + lane, blk = g >> pg;
+        if (g >= u.tile1 * kFewGroups || g >= groups) return kNowhere;
+        if (blk >= fullb) return kOpen;
+        const int p = table[blk];
+        return p >= 0 && p < c.num_pages ? p : kNowhere;
+      };
+      auto scales = [&](int p) -> float2 {
+        if (kWide || p < 0) return make_float2(1.f, 1.f);
+        return *reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2);
+      };
+      int pages = kNowhere, pages1 = kNowhere;
+      if (more) {
+        pages = lookup(0);
+        pages1 = lookup(8 < u.tile1 - u.tile0 ? 1 : 0);
+        job.tile0 = u.tile0;
+        job.tile1 = u.tile1;
+        job.groups = groups;
+        job.length = static_cast<int>(u.s.length);
+        job.seq = static_cast<int>(u.s.seq);
+        job.h = u.h;
+        job.hg = u.hg;
+        job.pos = static_cast<int>(u.s.start + u.tok0);
+        job.ntok = u.ntok;
+        job.row = static_cast<int>(u.s.row0 + u.tok0);
+        job.whole = u.whole;
+        job.first = u.first;
+        job.cta0 = static_cast<int>(u.cta0);
+        job.cta1 = static_cast<int>(u.cta1);
+        job.vref = paged_vref(c, u.s, u.h);
+      }
+      ok = mbar_wait_warp(&job_empty[k & 1], ((k >> 1) & 1u) ^ 1u, abort_flag);
+      if (!ok) break;
+      if (lane == 0) {
+        jobs[k & 1] = job;
+        mbar_arrive(&job_full[k & 1]);
+      }
+      __syncwarp();
+      if (!more) break;
+      const float log2_vref = __log2f(job.vref);
+      const int ntile = u.tile1 - u.tile0;
+      float2 sc = scales(pages);
+      for (int c0 = 0; ok && c0 < ntile; c0 += 8) {
+        const int pages2 = c0 + 16 < ntile ? lookup(c0 / 8 + 2) : kNowhere;  // two chunks ahead of their copies
+        const float2 sc1 = scales(pages1);
+        const float lv = v_shift(sc.y, log2_vref);
+        float4 meta = make_float4(to2 * sc.x, lv, ex2_approx(-lv), __int_as_float(pages));
+        for (int i = 0; ok && i < 8 && c0 + i < ntile; ++i, ++stages) {
+          const int slot = stages % NS;
+          ok = mbar_wait_warp(&empty[slot], ((stages / NS) & 1u) ^ 1u, abort_flag);
+          if (!ok) break;
+          const bool mine = (lane >> 2) == i;  // lanes 4 i .. 4 i + 3 have this stage's groups
+          const unsigned n = __popc(__ballot_sync(0xffffffffu, mine && pages >= 0));
+          if (mine) s_meta[slot * kFewGroups + (lane & 3)] = meta;
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], n * 2 * Cfg::kGroupBytes);
+          __syncwarp();
+          if (mine && pages >= 0) {
+            const int g = (u.tile0 + c0) * kFewGroups + lane;
+            const uint8_t* src = c.pages + (static_cast<int64_t>(pages) * c.kv_heads + u.h) * 2 * part_bytes +
+                                 (g & ((1 << pg) - 1)) * Cfg::kGroupBytes;
+            uint8_t* dst = ring + slot * Cfg::kStageBytes + (lane & 3) * 2 * Cfg::kGroupBytes;
+            bulk_load(dst, src, Cfg::kGroupBytes, &full[slot]);
+            bulk_load(dst + Cfg::kGroupBytes, src + part_bytes, Cfg::kGroupBytes, &full[slot]);
+          }
+          __syncwarp();
+        }
+        pages = pages1;
+        pages1 = pages2;
+        sc = sc1;
+      }
+    }
+    if (!ok) {
+      if (lane == 0) {
+        atomicOr(&g_paged_error, kErrWaitTimeout);
+        *abort_flag = 1;
+      }
+      // the copies in flight land before the CTA can exit (bounded)
+      for (uint32_t i = stages > NS ? stages - NS : 0; i < stages; ++i)
+        (void)mbar_wait(&full[i % NS], (i / NS) & 1u, nullptr);
+    }
+    return;
+  }
+
+  // ---------------------------------------------------------------- rows
+  const int grp = warp % kFewGroups, r0 = 8 * NB * (warp / kFewGroups);  // group of a stage; first row
+  uint32_t stages = 0, met = 0;
+  auto meet_all = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(meet);
+    ok = mbar_wait_warp(meet, met & 1u, abort_flag);
+    ++met;
+  };
   FewRows<D, TIER, NB> w;
-  PagedPart u;
-  while (paged_next<kFewTile>(c, st, pl, walk, u)) {
-    const PagedSeq& s = u.s;
-    const int64_t tok0 = u.tok0, h = u.h;
-    const int ntok = u.ntok, hg = u.hg;
-    const bool whole = u.whole;
-    const int64_t g0 = static_cast<int64_t>(u.tile0) * kFewWarps;
-    const int64_t groups = (u.reach + 15) / 16;
-    int64_t g1 = static_cast<int64_t>(u.tile1) * kFewWarps;
-    g1 = g1 < groups ? g1 : groups;
-
-    // rows of the unit: row r = token r / Gc, query head h G + hg Gc + r % Gc
-    auto row_token = [&](int r) { return r / pl.Gc; };
-    auto row_ok = [&](int r) { return r < pl.Gc * pl.TQ && r / pl.Gc < ntok && hg * pl.Gc + r % pl.Gc < pl.G; };
-    int64_t lim[NB][2];
+  for (uint32_t kjob = 0;; ++kjob) {
+    ok = mbar_wait_warp(&job_full[kjob & 1], (kjob >> 1) & 1u, abort_flag);
+    if (!ok) break;
+    const FewJob u = jobs[kjob & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&job_empty[kjob & 1]);
+    if (u.tile1 < 0) break;
+    // row r: token r / Gc, query head h G + hg Gc + r % Gc
+    auto row_ok = [&](int r) { return r < pl.Gc * pl.TQ && r / pl.Gc < u.ntok && u.hg * pl.Gc + r % pl.Gc < pl.G; };
+    int lim[NB][2];
     w.clear();
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int r = 8 * n + gq;
-      const bool ok = row_ok(r);
-      const int64_t row = s.row0 + tok0 + (ok ? row_token(r) : 0);
-      const int head = static_cast<int>(h) * pl.G + hg * pl.Gc + (ok ? r % pl.Gc : 0);
+      const int r = r0 + 8 * n + gq;
+      const bool there = row_ok(r);
+      const int64_t row = u.row + (there ? r / pl.Gc : 0);
+      const int head = u.h * pl.G + u.hg * pl.Gc + (there ? r % pl.Gc : 0);
       const uint4* src = reinterpret_cast<const uint4*>(q.p + row * q.ld + head * D + q4 * (D / 4));
 #pragma unroll
       for (int i = 0; i < KB / 2; ++i) {
-        const uint4 x = ok ? src[i] : make_uint4(0, 0, 0, 0);
+        const uint4 x = there ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
         w.q[n][4 * i] = x.x;
         w.q[n][4 * i + 1] = x.y;
         w.q[n][4 * i + 2] = x.z;
@@ -926,77 +1112,40 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int t = row_token(8 * n + 2 * q4 + j);
-        lim[n][j] = s.start + tok0 + (t < ntok ? t : ntok - 1) + 1;
+        const int t = (r0 + 8 * n + 2 * q4 + j) / pl.Gc;
+        lim[n][j] = u.pos + (t < u.ntok ? t : u.ntok - 1) + 1;
       }
     }
-    const int64_t sure = s.start + tok0 + 1;  // keys that every row sees
-    const int pg = c.page_shift - 4;          // groups per page, log2
-    const int64_t full = TIER == kFP16 ? c.max_pages : s.length >> c.page_shift;  // blocks in pages
-    const int32_t* table = c.table + s.seq * c.max_pages;
-    auto page_of = [&](int64_t g) -> int {
-      const int64_t blk = g >> pg;
-      if (g >= g1 || blk >= full) return -1;
-      const int p = table[blk];
-      return p >= 0 && p < c.num_pages ? p : -1;
-    };
-    const float vref = paged_vref(c, s, u.h);
-    const float log2_vref = __log2f(vref);
-    int64_t g = g0 + warp;
-    if constexpr (TIER != kFP16) {
-      const int64_t gfull = (full << pg) < g1 ? full << pg : g1;  // groups held in 8 bits
-      const int64_t bytes = c.page_size * D;
-      uint4 kq[D / 32], vq[D / 32];
-      float2 sc2 = make_float2(0.f, 0.f);
-      int page = page_of(g), next = page_of(g + kFewWarps);
-      auto load = [&](int64_t gg, int p, uint4 (&ku)[D / 32], uint4 (&vu)[D / 32], float2& f2) {
-        if (p < 0) return;
-        const uint8_t* kp = c.pages + (static_cast<int64_t>(p) * c.kv_heads + h) * 2 * bytes +
-                            (gg & ((1 << pg) - 1)) * 16 * D + lane * 16;
-        const uint8_t* vp = kp + bytes;
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) ku[i] = __ldg(reinterpret_cast<const uint4*>(kp + i * 512));
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) vu[i] = __ldg(reinterpret_cast<const uint4*>(vp + i * 512));
-        f2 = __ldg(reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + h) * 2));
+    const int sure = u.pos + 1;  // keys that every row sees
+    for (int tile = u.tile0; tile < u.tile1; ++tile, ++stages) {
+      const int slot = stages % NS, key0 = (tile * kFewGroups + grp) * 16;
+      ok = mbar_wait_warp(&full[slot], (stages / NS) & 1u, abort_flag);
+      if (!ok) break;
+      const float4 meta = s_meta[slot * kFewGroups + grp];
+      const int where = __float_as_int(meta.w);
+      auto taken = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
       };
-      if (g < gfull) load(g, page, kq, vq, sc2);
-      for (; g < gfull; g += kFewWarps) {
-        uint4 kn[D / 32], vn[D / 32];
-        float2 sn = make_float2(0.f, 0.f);
-        const int after = page_of(g + 2 * kFewWarps);
-        if (g + kFewWarps < gfull) load(g + kFewWarps, next, kn, vn, sn);
-        if (page >= 0) {
-          const float lv = v_shift(sc2.y, log2_vref);
-          w.codes(kq, vq, to2 * sc2.x, lv, ex2_approx(-lv), g * 16, g * 16 + 16 > sure, lim, gq);
+      const uint4* kp = reinterpret_cast<const uint4*>(ring + slot * Cfg::kStageBytes + grp * 2 * Cfg::kGroupBytes) + lane;
+      const bool edge = key0 + 16 > sure;
+      if (where >= 0) {
+        if constexpr (kWide)
+          w.wide(kp, kp + Cfg::kGroupBytes / 16, meta.x, meta.y, meta.z, key0, edge, u.length, lim, gq, q4, taken);
+        else
+          w.codes(kp, kp + Cfg::kGroupBytes / 16, meta.x, meta.y, meta.z, key0, edge, lim, gq, taken);
+      } else {
+        taken();
+        if (!kWide && where == kOpen) {
+          const int64_t off = ((tile * kFewGroups + grp) & ((1 << pg) - 1)) * 2 * D + lane;
+          const int blk = u.length >> c.page_shift;
+          w.wide(reinterpret_cast<const uint4*>(paged_open(c, u.seq, blk, u.h, 0)) + off,
+                 reinterpret_cast<const uint4*>(paged_open(c, u.seq, blk, u.h, 1)) + off, meta.x, meta.y, meta.z, key0, edge,
+                 u.length, lim, gq, q4, [] {});
         }
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          kq[i] = kn[i];
-          vq[i] = vn[i];
-        }
-        sc2 = sn;
-        page = next;
-        next = after;
-      }
-      if (g < g1) {  // the open block
-        const float lv = v_shift(1.f, log2_vref), inv = ex2_approx(-lv);
-        const uint4* ko = reinterpret_cast<const uint4*>(paged_open(c, s.seq, full, h, 0));
-        const uint4* vo = reinterpret_cast<const uint4*>(paged_open(c, s.seq, full, h, 1));
-        for (; g < g1; g += kFewWarps) {
-          const int64_t off = (g - (full << pg)) * 2 * D + lane;
-          w.wide(ko + off, vo + off, to2, lv, inv, g * 16, g * 16 + 16 > sure, s.length, lim, gq, q4);
-        }
-      }
-    } else {
-      for (; g < g1; g += kFewWarps) {
-        const int page = page_of(g);
-        if (page < 0) continue;
-        const uint4* kp = reinterpret_cast<const uint4*>(paged_block(c, page, h, 0)) + (g & ((1 << pg) - 1)) * 2 * D + lane;
-        const uint4* vp = reinterpret_cast<const uint4*>(paged_block(c, page, h, 1)) + (g & ((1 << pg) - 1)) * 2 * D + lane;
-        w.wide(kp, vp, to2, 0.f, 1.f, g * 16, g * 16 + 16 > sure, s.length, lim, gq, q4);
       }
     }
+    if (!ok) break;
 
     // the warps' rows together
 #pragma unroll
@@ -1009,85 +1158,127 @@ __global__ void __launch_bounds__(kFewThreads, NB == 1 ? 3 : 2)
           l += __shfl_xor_sync(0xffffffffu, l, o);
           t += __shfl_xor_sync(0xffffffffu, t, o);
         }
-        const int r = 8 * n + 2 * q4 + j;
-        if (gq == 0) {
-          s_st[warp][r][0] = w.m[n][j];
-          s_st[warp][r][1] = l;
-          s_st[warp][r][2] = t;
-        }
+        const int r = r0 + 8 * n + 2 * q4 + j;
+        if (gq == 0) s_st[grp * R + r] = make_float4(w.m[n][j], l, t, 0.f);
+        float* dst = s_o + (grp * R + r) * Cfg::kOutRow + gq * (D / 8);
 #pragma unroll
-        for (int i = 0; i < KB; ++i) {
-          s_o[warp][r][gq * (D / 8) + 2 * i] = w.o[n][i][j];
-          s_o[warp][r][gq * (D / 8) + 2 * i + 1] = w.o[n][i][2 + j];
-        }
+        for (int i = 0; i < KB; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(w.o[n][i][j], w.o[n][i][2 + j]);
       }
     }
-    __syncthreads();
-    // one row of results: (m, l, t) and the columns this thread sums
-    auto finish = [&](int r, int col, float L, float T, float O) {
-      const int64_t row = s.row0 + tok0 + row_token(r);
-      const int head = static_cast<int>(h) * pl.G + hg * pl.Gc + r % pl.Gc;
+    meet_all();
+    if (!ok) break;
+    // one row of results: (m, l, t) and four columns
+    auto finish = [&](int r, int col, float L, float T, const float (&O)[4]) {
+      const int64_t row = u.row + r / pl.Gc;
+      const int head = u.h * pl.G + u.hg * pl.Gc + r % pl.Gc;
       const bool some = L != 0.f;  // a row that sees no key: zeros
-      out[row * ldo + head * D + col] = __float2half_rn(some ? O * vref / L : 0.f);
-      if (col == 0 && H != nullptr)
-        H[row * heads + head] = some ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
+      const float f = some ? u.vref / L : 0.f;
+      uint2 x = make_uint2(0, 0);
+      if (some) x = make_uint2(pack2(O[0] * f, O[1] * f), pack2(O[2] * f, O[3] * f));
+      *reinterpret_cast<uint2*>(out + row * ldo + head * D + col) = x;
+      if (col == 0 && H != nullptr) H[row * heads + head] = some ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
     };
-    const int64_t first = u.cta0, last = u.cta1;
-    for (int i = tid; i < R * D; i += kFewThreads) {
-      const int r = i / D, col = i % D;
+    for (int i = tid; i < R * (D / 4); i += NT) {
+      const int r = i / (D / 4), col = i % (D / 4) * 4;
       if (!row_ok(r)) continue;
-      float M = kNegInf, L = 0.f, T = 0.f, O = 0.f;
+      float M = kNegInf, L = 0.f, T = 0.f, O[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < kFewWarps; ++k) M = fmaxf(M, s_st[k][r][0]);
+      for (int k = 0; k < kFewGroups; ++k) M = fmaxf(M, s_st[k * R + r].x);
 #pragma unroll
-      for (int k = 0; k < kFewWarps; ++k) {
-        const float mk = s_st[k][r][0], lk = s_st[k][r][1];
-        if (mk == kNegInf && lk == 0.f) continue;  // saw no key (NaN sums go on)
-        const float a = mk == kNegInf ? 1.f : ex2_approx(mk - M);
-        L += a * lk;
-        T += a * (s_st[k][r][2] + (mk == kNegInf ? 0.f : lk * (mk - M)));
-        O += a * s_o[k][r][col];
+      for (int k = 0; k < kFewGroups; ++k) {
+        const float4 x = s_st[k * R + r];
+        const float4 o = *reinterpret_cast<const float4*>(s_o + (k * R + r) * Cfg::kOutRow + col);
+        // a warp that saw no key adds nothing; NaN sums go on
+        const bool none = x.x == kNegInf && x.y == 0.f;
+        const float a = none ? 0.f : (x.x == kNegInf ? 1.f : ex2_approx(x.x - M));
+        L += a * x.y;
+        T += a * (x.z + (x.x == kNegInf ? 0.f : x.y * (x.x - M)));
+        O[0] += a * o.x;
+        O[1] += a * o.y;
+        O[2] += a * o.z;
+        O[3] += a * o.w;
       }
-      if (whole) {
+      if (u.whole) {
         finish(r, col, L, T, O);
       } else {
-        float* rec = part + ((2 * blockIdx.x + (u.first ? 1 : 0)) * R + r) * REC;
-        rec[4 + col] = O;
+        float* rec = part + ((2 * static_cast<int64_t>(blockIdx.x) + u.first) * R + r) * REC;
+        *reinterpret_cast<float4*>(rec + 4 + col) = make_float4(O[0], O[1], O[2], O[3]);
         if (col == 0) *reinterpret_cast<float4*>(rec) = make_float4(M, L, T, 0.f);
       }
     }
-    if (!whole) {
+    if (!u.whole) {
       __threadfence();
-      __syncthreads();
+      meet_all();
+      if (!ok) break;
       if (tid == 0) {
-        s_last = atomicAdd(&tickets[first], 1u) == static_cast<uint32_t>(last - first);
-        if (s_last) tickets[first] = 0;  // left as it was found
+        const uint32_t last = atomicAdd(&tickets[u.cta0], 1u) == static_cast<uint32_t>(u.cta1 - u.cta0);
+        if (last) tickets[u.cta0] = 0;  // left as it was found
         __threadfence();
+        *s_last = last;
       }
-      __syncthreads();
-      if (s_last) {
-        for (int i = tid; i < R * D; i += kFewThreads) {
-          const int r = i / D, col = i % D;
+      meet_all();
+      if (!ok) break;
+      if (*s_last) {
+        const int parts = u.cta1 - u.cta0 + 1;
+        auto rec_of = [&](int k, int r) -> const float* {
+          return part + ((2 * static_cast<int64_t>(u.cta0 + k) + (k == 0 ? 1 : 0)) * R + r) * REC;
+        };
+        // a warp per row: the parts' weights into shared memory (there are at most kRowRoom CTAs),
+        // l and t summed by lanes in a fixed order
+        for (int r = warp; r < R; r += Cfg::kWarps) {
           if (!row_ok(r)) continue;
-          float M = kNegInf, L = 0.f, T = 0.f, O = 0.f;
-          for (int64_t k = first; k <= last; ++k) {
-            const float* rec = part + ((2 * k + (k == first ? 1 : 0)) * R + r) * REC;
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec));
-            if (x.x == kNegInf && x.y == 0.f) continue;
-            const float o = __ldcg(rec + 4 + col);
-            const float mn = fmaxf(M, x.x);
-            const float a = M == kNegInf ? (mn == kNegInf ? 1.f : 0.f) : ex2_approx(M - mn);
-            const float e = x.x == kNegInf ? 1.f : ex2_approx(x.x - mn);
-            T = (M == kNegInf ? 0.f : a * (T + L * (M - mn))) + e * (x.z + (x.x == kNegInf ? 0.f : x.y * (x.x - mn)));
-            L = a * L + e * x.y;
-            O = a * O + e * o;
-            M = mn;
+          float M = kNegInf;
+          for (int k = lane; k < parts; k += 32) M = fmaxf(M, __ldcg(rec_of(k, r)));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+          float L = 0.f, T = 0.f;
+          for (int k = lane; k < parts; k += 32) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec_of(k, r)));
+            const bool none = x.x == kNegInf && x.y == 0.f;
+            const float a = none ? 0.f : (x.x == kNegInf ? 1.f : ex2_approx(x.x - M));
+            L += a * x.y;
+            T += a * (x.z + (x.x == kNegInf ? 0.f : x.y * (x.x - M)));
+            s_o[r * Cfg::kRowRoom + k] = a;
           }
-          finish(r, col, L, T, O);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            L += __shfl_xor_sync(0xffffffffu, L, o);
+            T += __shfl_xor_sync(0xffffffffu, T, o);
+          }
+          if (lane == 0) s_st[r] = make_float4(M, L, T, 0.f);
+        }
+      }
+      meet_all();
+      if (!ok) break;
+      if (*s_last) {
+        const int parts = u.cta1 - u.cta0 + 1;
+        const float* base0 = part + (2 * static_cast<int64_t>(u.cta0) + 1) * R * REC;
+        const float* base1 = part + 2 * static_cast<int64_t>(u.cta0 + 1) * R * REC;
+        for (int i = tid; i < R * (D / 4); i += NT) {
+          const int r = i / (D / 4), col = i % (D / 4) * 4;
+          if (!row_ok(r)) continue;
+          const float* wt = s_o + r * Cfg::kRowRoom;
+          const float4 x0 = __ldcg(reinterpret_cast<const float4*>(base0 + r * REC + 4 + col));
+          float O[4] = {wt[0] * x0.x, wt[0] * x0.y, wt[0] * x0.z, wt[0] * x0.w};
+#pragma unroll 4
+          for (int k = 1; k < parts; ++k) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(base1 + (static_cast<int64_t>(2 * (k - 1)) * R + r) * REC + 4 + col));
+            O[0] = fmaf(wt[k], x.x, O[0]);
+            O[1] = fmaf(wt[k], x.y, O[1]);
+            O[2] = fmaf(wt[k], x.z, O[2]);
+            O[3] = fmaf(wt[k], x.w, O[3]);
+          }
+          const float4 f = s_st[r];
+          finish(r, col, f.y, f.z, O);
         }
       }
     }
-    __syncthreads();  // the shared rows are free again
+    meet_all();  // the shared rows are free again
+    if (!ok) break;
+  }
+  if (!ok && lane == 0) {
+    atomicOr(&g_paged_error, kErrWaitTimeout);
+    *abort_flag = 1;
   }
 }
 

@@ -76,8 +76,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// where a group of 16 keys is, besides page p >= 0: nowhere (a hole, or past the tokens), in the open block
-constexpr int kNowhere = -1, kOpen = -2;
 // masked scores: far below any score, and their product with a scale (1e-25 at least) far below
 // any reference, but finite, so that 0 times their distance is 0
 constexpr float kMasked = -1e33f;
@@ -793,9 +791,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
 // The units that several CTAs shared: block (x, y) joins rows 32 y .. of the unit that begins in CTA
 // x's share and runs past it (joins[x], written by that CTA), its parts in the order of the
-// keys.  Warp gq sums the dimensions gq D/8 .. of a row per lane: every load is a full line, and
-// none waits for another but the first (l and m say whether O was written at all, and then
-// select, not branch).
+// keys.  Warp gq sums four of the dimensions gq D/8 .. of a row per lane (block z says which): every
+// load is a full line, and none waits for another (l and m say whether O was written at all,
+// and then select, not branch).
 template <int D>
 __global__ void __launch_bounds__(256)
     paged_join_kernel(const PagedPlan pl, const PagedJoin* __restrict__ joins, int heads, __half* __restrict__ out,
@@ -813,34 +811,27 @@ __global__ void __launch_bounds__(256)
   float M = kNegInf;
 #pragma unroll 4
   for (int k = u.cta0; k <= u.cta1; ++k) M = fmaxf(M, rec_of(k)[0]);
-  float L = 0.f, T = 0.f, o[D / 8];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i] = 0.f;
-#pragma unroll 2
+  const int i0 = blockIdx.z * 4;
+  float L = 0.f, T = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int k = u.cta0; k <= u.cta1; ++k) {
     const float* rec = rec_of(k);
     const float m = rec[0], l = rec[256], t = rec[512];
-    float x[D / 8];
+    float x[4];
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) x[i] = rec[(3 + 8 * i + gq) * 256];
+    for (int i = 0; i < 4; ++i) x[i] = rec[(3 + 8 * (i0 + i) + gq) * 256];
     const bool none = m == kNegInf && l == 0.f;  // a part that saw no key of the row
     const float a = none ? 0.f : (m == kNegInf ? 1.f : ex2_approx(m - M));
     L = fmaf(a, l, L);
     T = none ? T : fmaf(a, t + (m == kNegInf ? 0.f : l * (m - M)), T);
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) o[i] = none ? o[i] : fmaf(a, x[i], o[i]);
+    for (int i = 0; i < 4; ++i) o[i] = none ? o[i] : fmaf(a, x[i], o[i]);
   }
   const int64_t qrow = u.row + tok;
   const int head = u.h * pl.G + hd;
   const float f = L != 0.f ? u.vref / L : 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 8; i += 8) {
-    uint32_t x[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = pack2(o[i + 2 * k] * f, o[i + 2 * k + 1] * f);
-    *reinterpret_cast<uint4*>(out + qrow * ldo + head * D + gq * (D / 8) + i) = make_uint4(x[0], x[1], x[2], x[3]);
-  }
-  if (gq == 0 && H != nullptr) H[qrow * heads + head] = L != 0.f ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
+  *reinterpret_cast<uint2*>(out + qrow * ldo + head * D + gq * (D / 8) + i0) = make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
+  if (gq == 0 && i0 == 0 && H != nullptr) H[qrow * heads + head] = L != 0.f ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
 }
 
 }  // namespace ee
