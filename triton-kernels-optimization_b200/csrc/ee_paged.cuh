@@ -605,9 +605,28 @@ __device__ __forceinline__ PagedWalk paged_begin(const PagedArgs& c, const Paged
   };
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    const int64_t W = paged_total(c, st, pl, lane), n = count(W);
-    int64_t b = 0, rem = 0;
-    if (cta < n) paged_locate(c, st, pl, cta * W / n, lane, b, rem);
+    int64_t W, b = 0, rem = 0;
+    if (st.batch <= 32) {  // a sequence per lane: the total and the place from one round of loads
+      int64_t cost = 0;
+      if (lane < st.batch) {
+        const PagedSeq s = paged_seq(c, st, lane);
+        if (!s.ok) atomicOr(&g_paged_error, kErrPage);
+        cost = paged_cost(s, pl).chain * c.kv_heads * pl.hgroups;
+      }
+      const int64_t incl = warp_scan(cost, lane);
+      W = __shfl_sync(0xffffffffu, incl, 31);
+      const int64_t n = count(W);
+      if (cta < n) {
+        const int64_t x = cta * W / n;
+        const int k = __ffs(__ballot_sync(0xffffffffu, incl > x)) - 1;
+        b = k;
+        rem = x - __shfl_sync(0xffffffffu, incl - cost, k);
+      }
+    } else {
+      W = paged_total(c, st, pl, lane);
+      const int64_t n = count(W);
+      if (cta < n) paged_locate(c, st, pl, cta * W / n, lane, b, rem);
+    }
     if (lane == 0) {
       share[0] = W;
       share[1] = b;
@@ -679,13 +698,9 @@ __device__ __forceinline__ bool paged_next(const PagedArgs& c, const PagedStepAr
   }
   return false;
 }
-// reference of the V scales of a (sequence, KV head): its first page's
-__device__ __forceinline__ float paged_vref(const PagedArgs& c, const PagedSeq& s, int h) {
-  if (c.tier == kFP16 || s.length < c.page_size) return 1.f;
-  const int p = paged_page(c, s.seq, 0);
-  const float x = p >= 0 ? c.scale[(static_cast<int64_t>(p) * c.kv_heads + h) * 2 + 1] : 1.f;
-  return x > 0.f && x < __builtin_huge_valf() ? x : 1.f;
-}
+// Reference of a part's V scales, from its first group's: any number of their size will do, as
+// the part's O is multiplied by it at the end.
+__device__ __forceinline__ float v_reference(float vs) { return vs > 0.f && vs < __builtin_huge_valf() ? vs : 1.f; }
 
 // ----------------------------------------------------------------------------------
 // attention of few rows
@@ -902,7 +917,7 @@ struct __align__(16) FewJob {
   int seq, h, hg, pos;               // pos: position of the unit's first token
   int ntok, row, whole, first;       // tokens; its query row
   int cta0, cta1;
-  float vref, pad;
+  int pad[2];
 };
 
 template <int D, int TIER, int NB, int RS>
@@ -921,7 +936,7 @@ struct FewCfg {
   static constexpr int kRec = D + 4;  // a part's row: m, l, t, -, O
   // ring, rows of the warps, (m, l, t) of the warps, metadata, jobs, barriers
   static constexpr size_t kSmem = 128 + size_t(NS) * kStageBytes + kOutBytes + kFewGroups * R * 16 + NS * kFewGroups * 16 +
-                                  2 * sizeof(FewJob) + (2 * NS + 5) * 8 + 64;
+                                  2 * sizeof(FewJob) + (2 * NS + 5) * 8 + 64;  // (the last: share, flags, V references)
 };
 
 // CTAs of kWarps + 1 warps, two or three per SM.  The copying warp walks the CTA's share of the
@@ -955,6 +970,7 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
   int64_t* s_share = reinterpret_cast<int64_t*>(meet + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(s_share + 3);
   volatile uint32_t* s_last = reinterpret_cast<volatile uint32_t*>(s_share + 3) + 1;
+  volatile float* s_vref = reinterpret_cast<volatile float*>(s_share + 4);  // [4]: the others may be two jobs behind
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, q4 = lane & 3;
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
@@ -1019,7 +1035,6 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
         job.first = u.first;
         job.cta0 = static_cast<int>(u.cta0);
         job.cta1 = static_cast<int>(u.cta1);
-        job.vref = paged_vref(c, u.s, u.h);
       }
       ok = mbar_wait_warp(&job_empty[k & 1], ((k >> 1) & 1u) ^ 1u, abort_flag);
       if (!ok) break;
@@ -1029,9 +1044,11 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
       }
       __syncwarp();
       if (!more) break;
-      const float log2_vref = __log2f(job.vref);
       const int ntile = u.tile1 - u.tile0;
       float2 sc = scales(pages);
+      const float vref = v_reference(__shfl_sync(0xffffffffu, sc.y, 0));
+      const float log2_vref = __log2f(vref);
+      if (lane == 0) s_vref[k & 3] = vref;  // with the part's first stage
       for (int c0 = 0; ok && c0 < ntile; c0 += 8) {
         const int pages2 = c0 + 16 < ntile ? lookup(c0 / 8 + 2) : kNowhere;  // two chunks ahead of their copies
         const float2 sc1 = scales(pages1);
@@ -1146,8 +1163,9 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
       }
     }
     if (!ok) break;
+    const float vref = u.tile1 > u.tile0 ? s_vref[kjob & 3] : 1.f;
 
-    // the warps' rows together
+    // the warps' rows together, in units of V itself
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
 #pragma unroll
@@ -1162,7 +1180,7 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
         if (gq == 0) s_st[grp * R + r] = make_float4(w.m[n][j], l, t, 0.f);
         float* dst = s_o + (grp * R + r) * Cfg::kOutRow + gq * (D / 8);
 #pragma unroll
-        for (int i = 0; i < KB; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(w.o[n][i][j], w.o[n][i][2 + j]);
+        for (int i = 0; i < KB; ++i) *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(w.o[n][i][j] * vref, w.o[n][i][2 + j] * vref);
       }
     }
     meet_all();
@@ -1172,7 +1190,7 @@ __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, T
       const int64_t row = u.row + r / pl.Gc;
       const int head = u.h * pl.G + u.hg * pl.Gc + r % pl.Gc;
       const bool some = L != 0.f;  // a row that sees no key: zeros
-      const float f = some ? u.vref / L : 0.f;
+      const float f = some ? 1.f / L : 0.f;
       uint2 x = make_uint2(0, 0);
       if (some) x = make_uint2(pack2(O[0] * f, O[1] * f), pack2(O[2] * f, O[3] * f));
       *reinterpret_cast<uint2*>(out + row * ldo + head * D + col) = x;

@@ -85,7 +85,6 @@ struct PagedJoin {
   int64_t row;      // query row of its first token
   int h, hg, ntok;  // as in PagedPart
   int cta0, cta1;   // the CTAs; equal: none
-  float vref;
 };
 constexpr size_t kChunkJoinBytes = 48 * 1024;  // room for the joins of 1024 CTAs
 static_assert(sizeof(PagedJoin) * 1024 <= kChunkJoinBytes, "room for the joins");
@@ -96,11 +95,10 @@ struct __align__(16) ChunkJob {
   int n[2], nmax, tile0;          // key tiles of query tile 0 / 1, of the part; the part's first (nmax < 0: no more)
   int seq, h, hg, length;
   int pos, ntok, row, whole;      // position of the unit's first token; tokens; its query row; all of the unit
-  float vref, log2_vref;
-  int first, pad;
+  int first, pad[3];
 };
 __device__ __forceinline__ int chunk_tiles(int64_t reach) { return static_cast<int>((reach + kChunkTile - 1) / kChunkTile); }
-__device__ __forceinline__ ChunkJob chunk_job(const PagedArgs& c, const PagedPlan& pl, const PagedPart& u) {
+__device__ __forceinline__ ChunkJob chunk_job(const PagedPlan& pl, const PagedPart& u) {
   ChunkJob p;
   const int half = pl.TQ / 2;
   const int t0 = chunk_tiles(u.s.start + u.tok0 + (u.ntok < half ? u.ntok : half));
@@ -118,9 +116,7 @@ __device__ __forceinline__ ChunkJob chunk_job(const PagedArgs& c, const PagedPla
   p.row = static_cast<int>(u.s.row0 + u.tok0);
   p.whole = u.whole;
   p.first = u.first;
-  p.vref = paged_vref(c, u.s, u.h);
-  p.log2_vref = __log2f(p.vref);
-  p.pad = 0;
+  p.pad[0] = p.pad[1] = p.pad[2] = 0;
   return p;
 }
 
@@ -164,8 +160,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + NR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int64_t* s_share = reinterpret_cast<int64_t*>(tmem_slot + 2);
+  volatile float* s_vref = reinterpret_cast<volatile float*>(s_share + 3);  // [4] V reference of a part (the others may be two jobs behind)
   ChunkJob* jobs = reinterpret_cast<ChunkJob*>(reinterpret_cast<uint8_t*>(bars) + Cfg::kBarBytes - 2 * sizeof(ChunkJob));
-  static_assert((2 + 2 * NS + 2 * NV + 16 + 2 * NR) * 8 + 8 + 24 + 2 * sizeof(ChunkJob) <= Cfg::kBarBytes, "barrier region overflows");
+  static_assert((2 + 2 * NS + 2 * NV + 16 + 2 * NR) * 8 + 8 + 24 + 16 + 2 * sizeof(ChunkJob) <= Cfg::kBarBytes, "barrier region overflows");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -236,7 +233,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         more = paged_next<T>(c, st, pl, walk, part_u);
         ChunkJob job = {};
         job.nmax = -1;
-        if (more) job = chunk_job(c, pl, part_u);
+        if (more) job = chunk_job(pl, part_u);
         ok = mbar_wait_warp(&job_empty[k & 1], ((k >> 1) & 1u) ^ 1u, abort_flag);
         if (!ok) break;
         if (lane == 0) {
@@ -244,7 +241,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           mbar_arrive(&job_full[k & 1]);
           if (more && part_u.first && !part_u.whole)
             joins[blockIdx.x] = PagedJoin{part_u.s.row0 + part_u.tok0, part_u.h, part_u.hg, part_u.ntok,
-                                          static_cast<int>(part_u.cta0), static_cast<int>(part_u.cta1), job.vref};
+                                          static_cast<int>(part_u.cta0), static_cast<int>(part_u.cta1)};
         }
         __syncwarp();
       }
@@ -275,6 +272,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (kWide || p < 0) return make_float2(1.f, 1.f);
           return *reinterpret_cast<const float2*>(c.scale + (static_cast<int64_t>(p) * c.kv_heads + u.h) * 2);
         };
+        int p0 = lookup(0), p1 = lookup(1);  // page numbers a tile ahead of the copies
+        float2 sc = scales(p0);
+        const float vref = v_reference(__shfl_sync(0xffffffffu, sc.y, 0)), log2_vref = __log2f(vref);
+        if (lane == 0) s_vref[(njob - 1) & 3] = vref;  // with the part's first tile
         auto copy = [&](int j, int p, int which) {
           const uint8_t* src = c.pages + ((static_cast<int64_t>(p) * c.kv_heads + u.h) * 2 + which) * part_bytes +
                                (((u.tile0 + j) * 8 + lane) & ((1 << pg) - 1)) * (kGroupBytes * kHalves);
@@ -293,13 +294,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         };
         auto tell = [&](int j, int p, float2 sc) {
           if (lane >= 8) return;
-          const float lv = v_shift(sc.y, u.log2_vref);
+          const float lv = v_shift(sc.y, log2_vref);
           float4 m = make_float4(fmaxf(to2 * sc.x, 1e-25f), lv, ex2_approx(-lv), __int_as_float(p));
           if (p == kNowhere) m = make_float4(1e-25f, kMasked, 1.f, __int_as_float(p));
           sMeta[((kt + j) % kChunkMeta) * 8 + lane] = m;
         };
-        int p0 = lookup(0), p1 = lookup(1);  // page numbers a tile ahead of the copies
-        float2 sc = scales(p0);
         if (u.nmax > 0) {
           tell(0, p0, sc);
           __syncwarp();
@@ -731,7 +730,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       float* rec = part + (2 * static_cast<int64_t>(blockIdx.x) + (u.first ? 1 : 0)) * Cfg::kRec + w * T + row;
       if (n > 0) {
         tc_fence_after();
-        const float f = l != 0.f ? u.vref / l : 0.f;  // a row that sees no key: zeros
+        // O in units of V itself; a row that sees no key: zeros
+        const float vref = s_vref[(njob - 1) & 3], f = l != 0.f ? vref / l : 0.f;
         __half* dst = out + qrow * ldo + head * D;
 #pragma unroll
         for (int hh = 0; hh < D / 64; ++hh) {  // columns 64 hh ..: dimensions 8 hh .. of each gq's
@@ -758,8 +758,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           } else if (real) {
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-              rec[(3 + 64 * hh + k) * 256] = __uint_as_float(a[k]);
-              rec[(3 + 64 * hh + 32 + k) * 256] = __uint_as_float(b[k]);
+              rec[(3 + 64 * hh + k) * 256] = __uint_as_float(a[k]) * vref;
+              rec[(3 + 64 * hh + 32 + k) * 256] = __uint_as_float(b[k]) * vref;
             }
           }
         }
@@ -829,7 +829,7 @@ __global__ void __launch_bounds__(256)
   }
   const int64_t qrow = u.row + tok;
   const int head = u.h * pl.G + hd;
-  const float f = L != 0.f ? u.vref / L : 0.f;
+  const float f = L != 0.f ? 1.f / L : 0.f;
   *reinterpret_cast<uint2*>(out + qrow * ldo + head * D + gq * (D / 8) + i0) = make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
   if (gq == 0 && i0 == 0 && H != nullptr) H[qrow * heads + head] = L != 0.f ? 0.69314718055994531f * (__log2f(L) - T / L) : 0.f;
 }
