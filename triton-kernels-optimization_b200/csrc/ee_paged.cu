@@ -110,9 +110,11 @@ int run_attention(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& 
   pl.hgroups = (G + R - 1) / R;
   pl.Gc = (G + pl.hgroups - 1) / pl.hgroups;
   pl.TQ = R / pl.Gc;
-  pl.fixed = 2 * kFewTile;
-  // no CTA for less than four stages: shorter parts cost more in joining than they save
-  pl.min_cost = 4 * kFewTile;
+  // a part's start and end take about as long as four stages (48 ragged sequences: 90 us with
+  // two, 83 with four or six), and no CTA is started for less than two (one sequence of 777
+  // tokens: 20 us with eight, 16 with four, 15.5 with two)
+  pl.fixed = 4 * kFewTile;
+  pl.min_cost = 2 * kFewTile;
   if (R == 8) return run_few<D, TIER, 1, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
   if (R == 16) return run_few<D, TIER, 2, 1>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);
   if (R == 32) return run_few<D, TIER, 2, 2>(c, st, pl, q, heads, scale, out, ldo, H, tickets, part, s);

@@ -930,7 +930,10 @@ struct FewCfg {
   static constexpr int kStageBytes = 2 * kFewGroups * kGroupBytes;
   static constexpr int NS = kStageBytes > 24 * 1024 ? 2 : 48 * 1024 / kStageBytes;
   static constexpr int kOutRow = D + 4;
-  static constexpr int kCtas = NB == 1 ? 3 : (RS == 1 ? 2 : 1);  // per SM, by the launch bounds
+  // per SM, by the launch bounds: three leave 128 registers a thread, which D = 128 spills
+  // (48 sequences of up to 8000 tokens: 97 us with three, 90 with two; 16 x 8192 with D = 64:
+  // 20.5 with three, 21.8 with two)
+  static constexpr int kCtas = NB == 1 ? (D == 64 ? 3 : 2) : (RS == 1 ? 2 : 1);
   static constexpr int kRowRoom = kFewGroups * kOutRow > kCtas * 160 ? kFewGroups * kOutRow : kCtas * 160;
   static constexpr int kOutBytes = R * kRowRoom * 4;  // the groups' rows, then a weight per part
   static constexpr int kRec = D + 4;  // a part's row: m, l, t, -, O
