@@ -54,7 +54,7 @@ int run_append(const PagedArgs& c, const PagedStepArgs& st, const PagedRows& k, 
   int e = allow_smem<paged_append_kernel<D, TIER>>(paged_stage_bytes(128, D));
   if (e != 0) return e;
   const int64_t kv = block_slots(c, st) * c.kv_heads;
-  const int64_t qn = q.p == nullptr ? 0 : (st.rows * heads * (D / 16) + kPagedAppendThreads - 1) / kPagedAppendThreads;
+  const int64_t qn = q.p == nullptr ? 0 : (st.rows + kQTokens - 1) / kQTokens;
   return launch_pdl(paged_append_kernel<D, TIER>, dim3(static_cast<unsigned>(kv + qn)), dim3(kPagedAppendThreads),
                     paged_stage_bytes(static_cast<int>(c.page_size), D), s, c, st, k, v, cos, sin, ld_cs, q, heads, q_out,
                     ldqo, kv);

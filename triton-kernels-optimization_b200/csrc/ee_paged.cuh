@@ -129,23 +129,68 @@ __device__ __forceinline__ uint4 rope8(const uint4& x, const uint4& partner, boo
   }
   return o;
 }
-template <int D>
-__device__ __forceinline__ uint4 load_rotated(const __half* row, int d0, const __half* cs, const __half* sn) {
-  const uint4 x = *reinterpret_cast<const uint4*>(row + d0);
-  if (cs == nullptr) return x;
-  const bool low = d0 < D / 2;
-  const uint4 p = *reinterpret_cast<const uint4*>(row + (low ? d0 + D / 2 : d0 - D / 2));
-  return rope8(x, p, low, *reinterpret_cast<const uint4*>(cs + d0), *reinterpret_cast<const uint4*>(sn + d0));
+// Codes rn(fp32(x / s)) of 16 values, one byte each in order.  x * (1 / s) is within two fp32 steps
+// of the quotient (1 / s and the product are rounded once each), so its code is the same unless
+// a rounding boundary lies that near; only then (one warp in ten or less) the quotients are
+// computed.  int8: x (1 / s) + 1.5 2^23 + 128 rounds to an integer whose low byte is the code plus
+// 128; boundaries are the halves.  e4m3: boundaries have no bits set below the first four of
+// the mantissa, normal or not.
+template <int TIER>
+__device__ __forceinline__ uint4 quantise16(const float (&x)[16], float s, float inv) {
+  constexpr float kMagic = 12582912.f + 128.f;
+  uint32_t w[4];
+  if constexpr (TIER == kINT8) {
+    float r[16], far = 0.f;  // the rounded numbers; the largest distance from one
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      r[i] = fmaf(x[i], inv, kMagic);
+      far = fmaxf(far, fabsf(fmaf(x[i], inv, kMagic - r[i])));
+    }
+    if (!(far < 0.4999f)) {  // (NaN too: a block that is not finite)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float y = __fdiv_rn(x[i], s);
+        r[i] = (y == y ? y : 0.f) + kMagic;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = __byte_perm(__float_as_uint(r[4 * i]), __float_as_uint(r[4 * i + 1]), 0x0040);
+      const uint32_t b = __byte_perm(__float_as_uint(r[4 * i + 2]), __float_as_uint(r[4 * i + 3]), 0x0040);
+      w[i] = __byte_perm(a, b, 0x5410);
+    }
+  } else {
+    float y[16];
+    uint32_t near = ~0u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      y[i] = x[i] * inv;
+      const uint32_t z = (__float_as_uint(y[i]) + 4u) & 0x7FFFFu;
+      near = z < near ? z : near;
+    }
+    if (near <= 8u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = __fdiv_rn(x[i], s);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint16_t a, b;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(y[4 * i + 1]), "f"(y[4 * i]));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(y[4 * i + 3]), "f"(y[4 * i + 2]));
+      w[i] = static_cast<uint32_t>(a) | static_cast<uint32_t>(b) << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 constexpr int kPagedAppendThreads = 256;
+constexpr int kQTokens = 4;  // query rows per CTA
 // shared memory of an append CTA: the block's K and V rows, padded by 16 bytes
 __host__ __device__ constexpr size_t paged_stage_bytes(int page, int D) { return size_t(2) * page * (D + 8) * 2; }
 
-// One CTA per (touched block, KV head), then CTAs that rotate q (kPagedAppendThreads pairs of
-// eight values each).
+// One CTA per (touched block, KV head), then CTAs that rotate kQTokens rows of q.
 template <int D, int TIER>
-__global__ void __launch_bounds__(kPagedAppendThreads)
+__global__ void __launch_bounds__(kPagedAppendThreads, 4)
     paged_append_kernel(const PagedArgs c, const PagedStepArgs st, const PagedRows k, const PagedRows v,
                         const __half* __restrict__ cos, const __half* __restrict__ sin, int64_t ld_cs,
                         const PagedRows q, int heads, __half* q_out, int64_t ldqo, int64_t kv_ctas) {
@@ -156,24 +201,27 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   griddep_launch_dependents();
-  if (blockIdx.x >= kv_ctas) {  // q: a thread has both halves of its pairs, so q_out may be q
-    const int64_t i = (blockIdx.x - kv_ctas) * kPagedAppendThreads + tid;
-    const int64_t row = i / (heads * (VPR / 2));
-    if (row >= st.rows) return;
-    const int vec = static_cast<int>(i % (heads * (VPR / 2)));
-    const int h = vec / (VPR / 2), d0 = (vec % (VPR / 2)) * 8, d1 = d0 + D / 2;
-    const __half* src = q.p + row * q.ld + h * D;
-    uint4 lo = *reinterpret_cast<const uint4*>(src + d0), hi = *reinterpret_cast<const uint4*>(src + d1);
-    if (cos != nullptr) {
-      const __half* cr = cos + row * ld_cs;
-      const __half* sr = sin + row * ld_cs;
-      const uint4 x = rope8(lo, hi, true, *reinterpret_cast<const uint4*>(cr + d0), *reinterpret_cast<const uint4*>(sr + d0));
-      hi = rope8(hi, lo, false, *reinterpret_cast<const uint4*>(cr + d1), *reinterpret_cast<const uint4*>(sr + d1));
-      lo = x;
+  if (blockIdx.x >= kv_ctas) {  // q, kQTokens rows: a thread has both halves of its pairs, so q_out may be q
+    const int64_t row0 = (blockIdx.x - kv_ctas) * kQTokens;
+    const unsigned per = heads * (VPR / 2);
+    const unsigned items = per * static_cast<unsigned>(st.rows - row0 < kQTokens ? st.rows - row0 : kQTokens);
+    for (unsigned i = tid; i < items; i += kPagedAppendThreads) {
+      const int64_t row = row0 + i / per;
+      const unsigned vec = i % per;
+      const int h = vec / (VPR / 2), d0 = (vec % (VPR / 2)) * 8;
+      const uint4* src = reinterpret_cast<const uint4*>(q.p + row * q.ld + h * D + d0);
+      uint4 lo = src[0], hi = src[D / 16];
+      if (cos != nullptr) {
+        const uint4* cr = reinterpret_cast<const uint4*>(cos + row * ld_cs + d0);
+        const uint4* sr = reinterpret_cast<const uint4*>(sin + row * ld_cs + d0);
+        const uint4 x = rope8(lo, hi, true, __ldg(cr), __ldg(sr));
+        hi = rope8(hi, lo, false, __ldg(cr + D / 16), __ldg(sr + D / 16));
+        lo = x;
+      }
+      uint4* dst = reinterpret_cast<uint4*>(q_out + row * ldqo + h * D + d0);
+      dst[0] = lo;
+      dst[D / 16] = hi;
     }
-    __half* dst = q_out + row * ldqo + h * D;
-    *reinterpret_cast<uint4*>(dst + d0) = lo;
-    *reinterpret_cast<uint4*>(dst + d1) = hi;
     return;
   }
   const int64_t slot = blockIdx.x / c.kv_heads;
@@ -196,14 +244,47 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
   __half* sk = reinterpret_cast<__half*>(paged_smem);
   __half* sv = sk + P * LD;
 
-  // rows [r0, r1) of block x (new tokens) into the stage
+  float mk = 0.f, mv = 0.f;  // max |x| of the values that pass this thread
+  bool bad_k = false, bad_v = false;  // fmaxf drops NaN: carried apart
+  auto note = [](const uint4& x, float& m, bool& bad) {
+    const __half2* h = reinterpret_cast<const __half2*>(&x);
+    const __half2 a = __hmax2_nan(__hmax2_nan(__habs2(h[0]), __habs2(h[1])), __hmax2_nan(__habs2(h[2]), __habs2(h[3])));
+    const float2 f = __half22float2(a);
+    m = fmaxf(m, fmaxf(f.x, f.y));
+    bad = bad || f.x != f.x || f.y != f.y;
+  };
+  // rows [r0, r1) of the block at `base` (new tokens) into the stage.  A thread takes 8 values of
+  // a row's lower half and the 8 of its upper half that they are rotated with, all loads
+  // before the first store.
   auto stage_new = [&](int64_t base, int r0, int r1) {
-    for (int i = tid; i < (r1 - r0) * VPR; i += kPagedAppendThreads) {
-      const int t = r0 + i / VPR, d0 = (i % VPR) * 8;
+    constexpr int PV = VPR / 2;
+    for (int i = tid; i < (r1 - r0) * PV; i += kPagedAppendThreads) {
+      const int t = r0 + i / PV, d0 = (i % PV) * 8;
       const int64_t row = s.row0 + base + t - s.start;
-      *reinterpret_cast<uint4*>(sk + t * LD + d0) =
-          load_rotated<D>(k.p + row * k.ld + h * D, d0, cos == nullptr ? nullptr : cos + row * ld_cs, sin + row * ld_cs);
-      *reinterpret_cast<uint4*>(sv + t * LD + d0) = *reinterpret_cast<const uint4*>(v.p + row * v.ld + h * D + d0);
+      const uint4* kr = reinterpret_cast<const uint4*>(k.p + row * k.ld + h * D + d0);
+      const uint4* vr = reinterpret_cast<const uint4*>(v.p + row * v.ld + h * D + d0);
+      uint4 lo = __ldg(kr), hi = __ldg(kr + D / 16);
+      const uint4 v0 = __ldg(vr), v1 = __ldg(vr + D / 16);
+      if (cos != nullptr) {
+        const uint4* cr = reinterpret_cast<const uint4*>(cos + row * ld_cs + d0);
+        const uint4* sr = reinterpret_cast<const uint4*>(sin + row * ld_cs + d0);
+        const uint4 c0 = __ldg(cr), c1 = __ldg(cr + D / 16), s0 = __ldg(sr), s1 = __ldg(sr + D / 16);
+        const uint4 x = rope8(lo, hi, true, c0, s0);
+        hi = rope8(hi, lo, false, c1, s1);
+        lo = x;
+      }
+      uint4* kd = reinterpret_cast<uint4*>(sk + t * LD + d0);
+      uint4* vd = reinterpret_cast<uint4*>(sv + t * LD + d0);
+      kd[0] = lo;
+      kd[D / 16] = hi;
+      vd[0] = v0;
+      vd[D / 16] = v1;
+      if constexpr (TIER != kFP16) {
+        note(lo, mk, bad_k);
+        note(hi, mk, bad_k);
+        note(v0, mv, bad_v);
+        note(v1, mv, bad_v);
+      }
     }
   };
   // stage rows [r0, r1) to fp16 in page order at kd / vd
@@ -253,7 +334,9 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
       const __half* vo = paged_open(c, s.seq, blk, h, 1);
       for (int i = tid; i < t0 * VPR; i += kPagedAppendThreads) {
         const int t = i / VPR, d0 = (i % VPR) * 8;
-        *reinterpret_cast<uint4*>(sk + t * LD + d0) = *reinterpret_cast<const uint4*>(ko + page_k_offset<D, true>(t, d0));
+        const uint4 x = *reinterpret_cast<const uint4*>(ko + page_k_offset<D, true>(t, d0));
+        *reinterpret_cast<uint4*>(sk + t * LD + d0) = x;
+        note(x, mk, bad_k);
       }
       for (int i = tid; i < ((t0 + 15) >> 4) * 2 * D; i += kPagedAppendThreads) {
         const int g = i / (2 * D), u = i % (2 * D);
@@ -264,28 +347,15 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int tt = t + (e >> 2) * 8 + (e & 1);
-          if (tt < t0) sv[tt * LD + d0 + ((e >> 1) & 1)] = val[e];
+          if (tt < t0) {
+            sv[tt * LD + d0 + ((e >> 1) & 1)] = val[e];
+            mv = fmaxf(mv, fabsf(__half2float(val[e])));
+            bad_v = bad_v || __hisnan(val[e]);
+          }
         }
       }
     }
-    __syncthreads();
     if (complete && page >= 0) {
-      float mk = 0.f, mv = 0.f;
-      bool bad_k = false, bad_v = false;  // fmaxf drops NaN: carried apart
-      for (int i = tid; i < static_cast<int>(P) * VPR; i += kPagedAppendThreads) {
-        const int o = (i / VPR) * LD + (i % VPR) * 8;
-        const uint4 xk = *reinterpret_cast<const uint4*>(sk + o), xv = *reinterpret_cast<const uint4*>(sv + o);
-        const __half2* a = reinterpret_cast<const __half2*>(&xk);
-        const __half2* w = reinterpret_cast<const __half2*>(&xv);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 fa = __half22float2(a[e]), fw = __half22float2(w[e]);
-          mk = fmaxf(mk, fmaxf(fabsf(fa.x), fabsf(fa.y)));
-          mv = fmaxf(mv, fmaxf(fabsf(fw.x), fabsf(fw.y)));
-          bad_k = bad_k || fa.x != fa.x || fa.y != fa.y;
-          bad_v = bad_v || fw.x != fw.x || fw.y != fw.y;
-        }
-      }
       if (bad_k) mk = __builtin_huge_valf();  // a NaN makes the block's scale infinite, and its rows NaN
       if (bad_v) mv = __builtin_huge_valf();
 #pragma unroll
@@ -297,7 +367,7 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
         s_max[0][warp] = mk;
         s_max[1][warp] = mv;
       }
-      __syncthreads();
+      __syncthreads();  // the maxima, and the stage
       mk = s_max[0][0];
       mv = s_max[1][0];
 #pragma unroll
@@ -309,47 +379,50 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
       const float ks = __fdiv_rn(mk, kTop), vs = __fdiv_rn(mv, kTop);
       if (tid == 0) *reinterpret_cast<float2*>(c.scale + (static_cast<int64_t>(page) * c.kv_heads + h) * 2) = make_float2(ks, vs);
       const float dk = ks > 0.f ? ks : 1.f, dv = vs > 0.f ? vs : 1.f;  // an all-zero block: scale 0, codes 0
-      auto code2 = [&](float a, float w) -> uint32_t {  // two codes, low byte first
-        if constexpr (TIER == kINT8) {
-          const int ia = __float2int_rn(fminf(fmaxf(a, -127.f), 127.f)), iw = __float2int_rn(fminf(fmaxf(w, -127.f), 127.f));
-          return static_cast<uint32_t>(ia + 128) | static_cast<uint32_t>(iw + 128) << 8;
-        } else {
-          uint16_t o;
-          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(o) : "f"(w), "f"(a));
-          return o;
-        }
-      };
+      const float ik = 1.f / dk, iv = 1.f / dv;
       uint8_t* kd = paged_block(c, page, h, 0);
       uint8_t* vd = paged_block(c, page, h, 1);
       const int units = static_cast<int>(P) * D / 16;
       for (int i = tid; i < units; i += kPagedAppendThreads) {
         const int g = i / D, u = i % D;  // D units per group of 16 tokens
         const int ln = u & 31, gq = ln >> 2, q4 = ln & 3;
+        float x[16];
         {  // K: 16 dimensions of one token
           const int half = u / 32 / (D / 64), piece = u / 32 % (D / 64);
-          const __half* src = sk + (16 * g + 8 * half + gq) * LD + q4 * (D / 4) + piece * 16;
-          uint32_t w[4];
+          const uint4* src = reinterpret_cast<const uint4*>(sk + (16 * g + 8 * half + gq) * LD + q4 * (D / 4) + piece * 16);
+          const uint4 a = src[0], b = src[1];
+          const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = __half22float2(reinterpret_cast<const __half2*>(src)[2 * e]);
-            const float2 z = __half22float2(reinterpret_cast<const __half2*>(src)[2 * e + 1]);
-            w[e] = code2(__fdiv_rn(a.x, dk), __fdiv_rn(a.y, dk)) | code2(__fdiv_rn(z.x, dk), __fdiv_rn(z.y, dk)) << 16;
+          for (int e = 0; e < 8; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            x[2 * e] = f.x;
+            x[2 * e + 1] = f.y;
           }
-          *reinterpret_cast<uint4*>(kd + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(kd + i * 16) = quantise16<TIER>(x, dk, ik);
         }
         {  // V: four dimensions of four tokens
-          const int d0 = gq * (D / 8) + 4 * (u >> 5);
-          const __half* src = sv + (16 * g + 2 * q4) * LD + d0;
-          uint32_t w[4];
+          const __half* src = sv + (16 * g + 2 * q4) * LD + gq * (D / 8) + 4 * (u >> 5);
+          float2 f[4][2];  // tokens 0, 1, 8, 9
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {  // word: mb = e >> 1, th = e & 1
-            const __half* x = src + (e & 1) * 8 * LD + (e >> 1) * 2;
-            w[e] = code2(__fdiv_rn(__half2float(x[0]), dv), __fdiv_rn(__half2float(x[LD]), dv)) |
-                   code2(__fdiv_rn(__half2float(x[1]), dv), __fdiv_rn(__half2float(x[LD + 1]), dv)) << 16;
+          for (int e = 0; e < 4; ++e) {
+            const uint2 r = *reinterpret_cast<const uint2*>(src + ((e >> 1) * 8 + (e & 1)) * LD);
+            f[e][0] = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+            f[e][1] = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
           }
-          *reinterpret_cast<uint4*>(vd + i * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // word: dimensions 2 (e >> 1), + 1, tokens 8 (e & 1), + 1
+            const float2 t0 = f[2 * (e & 1)][e >> 1], t1 = f[2 * (e & 1) + 1][e >> 1];
+            x[4 * e] = t0.x;
+            x[4 * e + 1] = t1.x;
+            x[4 * e + 2] = t0.y;
+            x[4 * e + 3] = t1.y;
+          }
+          *reinterpret_cast<uint4*>(vd + i * 16) = quantise16<TIER>(x, dv, iv);
         }
       }
+    }
+    else {
+      __syncthreads();
     }
     // the fp16 rows of the sequence's last two blocks.  A later block whose slot holds the
     // tokens that the first block has yet to read is written by the first block's CTA, after
