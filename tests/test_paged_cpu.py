@@ -145,7 +145,7 @@ def test_tensor_checks(pkg):
     c.kv_heads, c.head_dim = 2, 64
     st = c.step([0], counts=[3])
     x = torch.zeros(3, 128, dtype=torch.float16)
-    c.device = torch.device("cuda:0")
+    c.device, c._index = torch.device("cuda:0"), 0
     for call in (lambda: c.append(x, x, st), lambda: c.attention(x, st)):
         with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
             call()

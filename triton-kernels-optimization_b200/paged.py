@@ -81,6 +81,8 @@ class PagedKVCache:
         self.device = torch.device(device)
         self.memory = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.device = self.memory.device
+        self._index = self.device.index
+        self._entry: Dict[str, object] = {}  # the library's entry points in use
         self.c = _PagedCacheC()
         self._ref = ctypes.byref(self.c)
         with torch.cuda.device(self.device):
@@ -174,13 +176,13 @@ class PagedKVCache:
 
     # A decode step is launch-bound: its host side checks with plain comparisons, formats a
     # message only when one fails, and enters the cache's device only when it is not the
-    # current one (append and attention of one token: 15 and 11 us of host time, from 25 and 26).
+    # current one.
     def _rows(self, x: torch.Tensor, name: str, rows: int, width: int) -> int:
         """Checks fp16 rows [rows, width] on the cache's device; their row stride."""
-        if x.get_device() != self.device.index:
-            raise RuntimeError(f"{name} must be a CUDA tensor on {self.device}")
         if x.dtype is not torch.float16 or x.shape != (rows, width):
             raise RuntimeError(f"{name} must be fp16 [{rows}, {width}]")
+        if x.get_device() != self._index:
+            raise RuntimeError(f"{name} must be a CUDA tensor on {self.device}")
         ld, col = x.stride()
         if col != 1 and width > 1:
             raise RuntimeError(f"{name} needs unit column stride")
@@ -189,12 +191,17 @@ class PagedKVCache:
 
     def _launch(self, name: str, *args) -> None:
         """One call on the cache's device and torch's current stream there (the last argument)."""
-        index = self.device.index
-        if torch.cuda.current_device() == index:
-            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        index = self._index
+        fn = self._entry.get(name)
+        if fn is None:
+            fn = self._entry[name] = getattr(_lib.load(), name)
+        if torch._C._cuda_getDevice() == index:
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         else:
             with torch.cuda.device(self.device):
-                call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+                status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            _lib.check(status, name)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, step: PagedStep, cos: Optional[torch.Tensor] = None,
                sin: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
@@ -245,7 +252,7 @@ class PagedKVCache:
         ldy = wide if out is None else self._rows(out, "out", n, wide)
         H = torch.empty((n, heads), dtype=torch.float32, device=self.device)
         # one workspace per stream: calls on different streams may run side by side
-        stream = torch._C._cuda_getCurrentRawStream(self.device.index)
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
         ws = self._ws.get(stream)
         if ws is None:  # zeroed once; the kernel leaves its head zero
             ws = self._ws[stream] = torch.zeros(_lib.load().ee_paged_workspace_bytes(self._ref), dtype=torch.uint8,
@@ -256,10 +263,10 @@ class PagedKVCache:
         return y, H
 
     def read(self, span: PagedStep):
-        """(k, v) fp16 [rows, kv_heads * head_dim] of a span: the values the cache stands for."""
+        """(k, v) fp16 [rows, kv_heads * head_dim] of a span: the values the cache stands for
+        (two halves of one allocation)."""
         width = self.kv_heads * self.head_dim
-        k = torch.empty((span.rows, width), dtype=torch.float16, device=self.device)
-        v = torch.empty((span.rows, width), dtype=torch.float16, device=self.device)
+        k, v = torch.empty((2, span.rows, width), dtype=torch.float16, device=self.device).unbind()
         self._launch("ee_paged_read", self._ref, span.ref, k.data_ptr(), width, v.data_ptr(), width)
         return k, v
 
