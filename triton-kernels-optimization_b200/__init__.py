@@ -22,6 +22,7 @@ from .dispatch import (
     tier_of,
 )
 from .engine import CubinEngine, DecoderEngine, GatedLayerEngine
+from .serve import PagedLlama
 from .llama import EntropyDispatchedLlamaBlock, build_dispatched_llama, dispatched_forward, eval_dispatched
 from .kernels import (
     SwiGLUPack,

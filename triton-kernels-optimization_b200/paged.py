@@ -164,6 +164,13 @@ class PagedKVCache:
         self._upload()
         return PagedStep(seqs, starts, counts, ends, self.device)
 
+    def share(self, step: PagedStep) -> None:
+        """Hands out the pages of a step that another cache made (the layers of a model advance
+        together: one step's arrays serve all their caches)."""
+        for s, e in zip(step.seqs, step.lengths):
+            self.reserve(s, e)
+        self._upload()
+
     def span(self, seqs: Sequence[int], starts: Sequence[int], counts: Sequence[int]) -> PagedStep:
         """Tokens ``starts[b] ..`` of sequences as they are cached, for ``read``."""
         seqs = [self._seq(s) for s in seqs]

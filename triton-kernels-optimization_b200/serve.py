@@ -1,0 +1,98 @@
+"""Serving loop of the dispatched Llama blocks over paged KV caches: prompts of different
+lengths enter in chunks, every step advances all sequences at once, and each token's MLP
+runs in the tier of its own attention entropy.
+
+    blocks, d = build_dispatched_llama(model, 0.41, 1.68, routing="token", attention="flash")
+    serve = PagedLlama(model, blocks, d, max_seqs=8, num_pages=1024)
+    texts = serve.generate([[1, 15, 7], [1, 9]], max_new_tokens=32)
+"""
+from __future__ import annotations
+
+from typing import List, Optional, Sequence
+
+import torch
+
+from .dispatch import PrecisionTier
+from .kernels import _require, add_rmsnorm, linear_f16
+from .paged import PagedKVCache, PagedStep
+
+
+class PagedLlama:
+    """A transformers Llama model's ``blocks`` (``build_dispatched_llama`` with
+    ``routing="token"``, ``attention="flash"``) with a ``PagedKVCache`` per layer."""
+
+    def __init__(self, model, blocks, dispatcher, max_seqs: int, num_pages: int, page_size: int = 64,
+                 max_pages: Optional[int] = None, tier: PrecisionTier = PrecisionTier.INT8):
+        _require(len(blocks) > 0 and all(b.attention == "flash" and b.routing == "token" and not b.route_all
+                                         for b in blocks),
+                 "the blocks must be built with routing='token', attention='flash' and without route_all")
+        self.model, self.blocks, self.dispatcher = model, blocks, dispatcher
+        a = blocks[0].self_attn
+        _require(all(getattr(a, n).bias is None for n in ("q_proj", "k_proj", "v_proj", "o_proj")),
+                 "the attention's projections must have no bias")
+        kv_heads = a.k_proj.out_features // a.head_dim
+        self.device = a.q_proj.weight.device
+        self.caches = [PagedKVCache(max_seqs, num_pages, page_size, kv_heads, a.head_dim, max_pages, tier, self.device)
+                       for _ in blocks]
+
+    def release(self, seq: int) -> None:
+        for c in self.caches:
+            c.release(seq)
+
+    def _layer(self, block, cache: PagedKVCache, hidden: torch.Tensor, step: PagedStep, cos, sin) -> torch.Tensor:
+        a = block.self_attn
+        x = add_rmsnorm(hidden, block.input_layernorm.weight, block.input_layernorm.variance_epsilon)
+        q, k, v = linear_f16(x, block.qkv_weight()).split(block._qkv_split, dim=-1)
+        q = cache.append(k, v, step, cos=cos, sin=sin, q=q)
+        out, entropy = cache.attention(q, step, a.scaling)
+        block.token_entropy = entropy.mean(dim=1)  # routes the token's MLP
+        x, residual = add_rmsnorm(linear_f16(out, a.o_proj.weight), block.post_attention_layernorm.weight,
+                                  block.post_attention_layernorm.variance_epsilon, residual=hidden)
+        return residual + block._mlp_per_token(x, self.dispatcher)
+
+    @torch.no_grad()
+    def forward(self, ids: Sequence[Sequence[int]], seqs: Sequence[int]) -> torch.Tensor:
+        """Appends ``ids[b]`` to sequence ``seqs[b]``; logits [rows, vocab] of all new tokens,
+        sequence after sequence."""
+        counts = [len(x) for x in ids]
+        # each layer's cache hands out its own pages; the step's arrays serve all of them
+        step = self.caches[0].step(seqs, counts=counts)
+        for c in self.caches[1:]:
+            c.share(step)
+        m = self.model.model
+        tokens = torch.tensor([t for x in ids for t in x], dtype=torch.long, device=self.device)
+        pos = torch.tensor([[a + i for a, n in zip(step.starts, counts) for i in range(n)]], dtype=torch.long,
+                           device=self.device)
+        hidden = m.embed_tokens(tokens).to(torch.float16)
+        cos, sin = (t[0].to(torch.float16) for t in m.rotary_emb(hidden[None], pos))
+        for block, cache in zip(self.blocks, self.caches):
+            hidden = self._layer(block, cache, hidden, step, cos, sin)
+        return self.model.lm_head(m.norm(hidden))
+
+    @torch.no_grad()
+    def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, chunk: int = 2048) -> List[List[int]]:
+        """Greedy continuations of the prompts (sequences 0 .. len(prompts) - 1, released at the
+        end): at most ``chunk`` prompt tokens of a sequence per step."""
+        _require(len(prompts) <= self.caches[0].max_seqs and all(len(p) > 0 for p in prompts),
+                 "at most max_seqs prompts, none of them empty")
+        _require(max_new_tokens >= 1 and chunk >= 1, "max_new_tokens and chunk must be >= 1")
+        seqs = list(range(len(prompts)))
+        _require(not any(self.caches[0].lengths[s] for s in seqs), "the prompts' sequences are in use")
+        out: List[List[int]] = [[] for _ in prompts]
+        waiting = [list(p) for p in prompts]  # tokens of each sequence that are not cached yet
+        try:
+            while any(len(o) < max_new_tokens for o in out):
+                active = [s for s in seqs if len(out[s]) < max_new_tokens]
+                ids = [waiting[s][:chunk] for s in active]
+                logits = self.forward(ids, active)
+                last = torch.tensor([len(x) for x in ids]).cumsum(0) - 1
+                best = logits[last.to(self.device)].argmax(dim=-1).tolist()
+                for s, x, token in zip(active, ids, best):
+                    waiting[s] = waiting[s][len(x):]
+                    if not waiting[s]:  # the prompt is in: the sequence goes on with its own tokens
+                        out[s].append(token)
+                        waiting[s] = [token]
+        finally:
+            for s in seqs:
+                self.release(s)
+        return out
