@@ -509,9 +509,10 @@ EE_API int ee_paged_read(const ee_paged_cache* cache, const ee_paged_step* step,
 /* Causal attention of the step's query rows (fp16 q [rows, heads * head_dim], rotated; heads a
  * multiple of kv_heads) after their append: the row at position p sees keys 0 .. p.  out fp16
  * [rows, heads * head_dim] = softmax(scale q k) v, H (nullable, fp32 [rows, heads]) the entropy
- * of each softmax row in nats; a row that sees no key gives zeros.  One launch, whatever the
- * lengths: the keys are dealt to the CTAs in even shares, and a unit's last CTA joins its
- * parts in a fixed order (the same bits every time).  workspace: ee_paged_workspace_bytes, its
+ * of each softmax row in nats; a row that sees no key gives zeros; rows of a step entry
+ * outside the cache are not written; out may not overlap q.  One or two launches, whatever the
+ * lengths: the keys are dealt to the CTAs in even shares, and the parts of rows whose keys
+ * several CTAs share are joined in a fixed order (the same bits every time).  workspace: ee_paged_workspace_bytes, its
  * first ee_paged_workspace_head_bytes() zeroed once (every call leaves them zero); one
  * workspace serves one call at a time. */
 EE_API size_t ee_paged_workspace_bytes(const ee_paged_cache* cache);
