@@ -20,6 +20,14 @@
 // 64 vb + 32 pi + 2 q4 + {0, 1, 8, 9, 16, 17, 24, 25} (P is stored alike).
 // Scales: K's multiplies S in fp32 with the softmax scale; V's raises the exponent of P
 // (v_shift), so P is rounded to fp16 once, with it.
+// What bounds it: 2048 tokens over 14000 (INT8, 32 / 8 heads of 128) take 712 us, 708 TFLOP/s, 0.41
+// of cuBLAS; tensor pipe 34 %, MUFU 35 %, issue 42 %, DRAM 1 %.  Taken apart (variants that leave
+// work out): no MMAs 603 us, no exponentials 700, no entropy sums 695, no maximum 687, no
+// conversion of the keys 679, nothing between the barriers 334, the barriers and the MMAs 429.
+// So no unit is short: it is the chain of one tile, S - softmax - P - P V with its hand-offs, in
+// two warps per scheduler.  Tried and not kept: two threads per row (788: the hand-over of the
+// maximum costs more than it hides), the maximum taken after the exponentials (1038: spills),
+// keys converted before their stage is free (728), other registers splits (710 - 730).
 // Every wait is bounded; on expiry the CTA records the error word, drains its MMAs, frees
 // TMEM and exits.
 //
@@ -631,35 +639,39 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tc_fence_after();
         const int seen = u.pos + tok + 1 - (u.tile0 + j) * T;
         const int lim = !real || seen > T ? T : (seen < 0 ? 0 : seen);
-        uint32_t r[4][32];
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tmem_ld32(t_s + 32 * k, r[k]);
-        tmem_ld_wait(r[0]);
-        regs_after_wait(r[1]);
-        regs_after_wait(r[2]);
-        regs_after_wait(r[3]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[w]);  // S_w is in registers: the next S may land
-        auto S = [&](int i) -> float { return __uint_as_float(r[i >> 5][i & 31]); };
-        if (!__all_sync(0xffffffffu, lim >= T)) {
-#pragma unroll
-          for (int i = 0; i < T; ++i)
-            if (i >= lim) r[i >> 5][i & 31] = __float_as_uint(kMasked);
-        }
+        const bool edge = !__all_sync(0xffffffffu, lim >= T);
         const float4* meta = sMeta + ((kt + j) % kChunkMeta) * 8;
-        float mt = kNegInf;
+        // The scores are read twice, 32 columns at a time, once for the row's maximum and once for
+        // its exponentials, in loops that stay rolled: unrolled over the tile, the code of the
+        // roles on a scheduler runs out of its instruction cache (5 ragged chunks: 90.5 us
+        // unrolled, 88.0 rolled; 2048 over 14000: 712 and 716; unrolled with two reads 831).
+        uint32_t r[32];
+        auto S = [&](int i) -> float { return __uint_as_float(r[i]); };
+        auto load = [&](int k) {
+          __syncwarp();
+          tmem_ld32(t_s + 32 * k, r);
+          tmem_ld_wait(r);
+          if (edge) {
 #pragma unroll
-        for (int gr = 0; gr < 8; ++gr) {
-          float a = fmaxf(S(16 * gr), S(16 * gr + 1)), b = fmaxf(S(16 * gr + 2), S(16 * gr + 3));
-#pragma unroll
-          for (int i = 4; i < 16; i += 4) {
-            a = fmaxf(a, fmaxf(S(16 * gr + i), S(16 * gr + i + 1)));
-            b = fmaxf(b, fmaxf(S(16 * gr + i + 2), S(16 * gr + i + 3)));
+            for (int i = 0; i < 32; ++i)
+              if (32 * k + i >= lim) r[i] = __float_as_uint(kMasked);
           }
-          const float4 f = meta[gr];
-          mt = fmaxf(mt, fmaf(fmaxf(a, b), f.x, f.y));
+        };
+        float mt = kNegInf;
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          load(k);
+#pragma unroll
+          for (int gr = 0; gr < 2; ++gr) {
+            float a = fmaxf(S(16 * gr), S(16 * gr + 1)), b = fmaxf(S(16 * gr + 2), S(16 * gr + 3));
+#pragma unroll
+            for (int i = 4; i < 16; i += 4) {
+              a = fmaxf(a, fmaxf(S(16 * gr + i), S(16 * gr + i + 1)));
+              b = fmaxf(b, fmaxf(S(16 * gr + i + 2), S(16 * gr + i + 3)));
+            }
+            const float2 f = *reinterpret_cast<const float2*>(meta + 2 * k + gr);
+            mt = fmaxf(mt, fmaf(fmaxf(a, b), f.x, f.y));
+          }
         }
         if (lim <= 0 || mt < 0.1f * kMasked) mt = kNegInf;  // sees no key of this tile
         float alpha = 1.f;
@@ -693,12 +705,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
         }
         const float mu = m == kNegInf ? 0.f : m;
-#pragma unroll
+#pragma unroll 1
         for (int sp = 0; sp < 4; ++sp) {
+          load(sp);
+          if (sp == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[w]);  // S_w is read: the next S may land
+          }
           uint32_t pk[2][8];
 #pragma unroll
           for (int ga = 0; ga < 2; ++ga) {
-            const int c0 = 32 * sp + 16 * ga;
+            const int c0 = 16 * ga;
             const float4 f = meta[2 * sp + ga];
             const float2 ks2 = make_float2(f.x, f.x), nb2 = make_float2(f.y - mu, f.y - mu);
             float2 sum = make_float2(0.f, 0.f), dot = make_float2(0.f, 0.f);
