@@ -178,7 +178,7 @@ def test_one_token_attention(pkg, cuda, tier, d, P, hk, hq):
 
 @pytest.mark.parametrize("tier", [0, 1, 2])
 @pytest.mark.parametrize("d,P,hk,hq", [(128, 16, 2, 8), (64, 32, 4, 4), (128, 64, 1, 7), (64, 128, 2, 6),
-                                       (128, 128, 1, 40), (64, 64, 1, 3)])
+                                       (128, 128, 1, 40), (64, 64, 1, 3), (64, 16, 1, 160)])
 @torch.no_grad()
 def test_chunk_attention(pkg, cuda, tier, d, P, hk, hq):
     """Chunks from one token to several tiles, from position 0 and over a cache, one long one
@@ -453,3 +453,47 @@ def test_steps_that_do_not_fit_the_cache_are_left_alone(pkg, cuda):
             pkg._lib.device_check()
         same = c.memory == before
         assert bool(same.all())
+
+
+@torch.no_grad()
+def test_attention_of_earlier_positions(pkg, cuda):
+    """Queries at positions before the sequence's end: its later tokens are cached and not seen."""
+    P, hk, hq, d, e = 32, 2, 8, 128, 500
+    g = torch.Generator(device=cuda).manual_seed(8)
+    k, v = _data(g, cuda, e, hk, d)
+    for tier in (0, 2):
+        c = _cache(pkg, cuda, [e], P, hk, d, tier)
+        c.append(k, v, c.step([0], counts=[e]))
+        for start, n in ((37, 1), (63, 3), (100, 90)):
+            q = torch.randn(n, hq * d, generator=g, device=cuda).half()
+            out, H = c.attention(q, c.span([0], [start], [n]))
+            _ok(pkg)
+            K, V = _held(k.view(e, hk, d), tier, P), _held(v.view(e, hk, d), tier, P)
+            _check(out, H, 0, n, _attend64(q.view(n, hq, d), K, V, start, d ** -0.5), hq, d)
+
+
+@torch.no_grad()
+def test_workspace_after_an_error(pkg, cuda):
+    """After device_check reported, the workspace's head is zeroed before its next use."""
+    P, hk, hq, d, e = 16, 2, 8, 64, 3000
+    g = torch.Generator(device=cuda).manual_seed(9)
+    k, v = _data(g, cuda, e, hk, d)
+    c = _cache(pkg, cuda, [e], P, hk, d, 1)
+    c.append(k, v, c.step([0], counts=[e]))
+    q = torch.randn(1, hq * d, generator=g, device=cuda).half()
+    st = c.step([0], starts=[e - 1])
+    want = c.attention(q, st)
+    (ws, _), = c._ws.values()
+    head = pkg.load_library().ee_paged_workspace_head_bytes()
+    torch.cuda.synchronize()
+    assert not ws[:head].any()
+    ws[:head] = 1  # as a kernel that gave up might leave it
+    st.arrays[0] = 7  # no such sequence: the error word
+    c.read(st)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="EE_ERR_DEVICE"):
+        pkg._lib.device_check()
+    st.arrays[0] = 0
+    got = c.attention(q, st)
+    _ok(pkg)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

@@ -95,7 +95,7 @@ class PagedKVCache:
         self._pages: List[List[int]] = [[] for _ in range(self.max_seqs)]
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._changed: Dict[int, int] = {}  # table entries not on the device yet
-        self._ws: Dict[int, torch.Tensor] = {}  # workspace of each stream
+        self._ws: Dict[int, list] = {}  # workspace of each stream, and the error count it was zeroed at
 
     # ------------------------------------------------------------------ pages
     @property
@@ -260,10 +260,14 @@ class PagedKVCache:
         H = torch.empty((n, heads), dtype=torch.float32, device=self.device)
         # one workspace per stream: calls on different streams may run side by side
         stream = torch._C._cuda_getCurrentRawStream(self._index)
-        ws = self._ws.get(stream)
-        if ws is None:  # zeroed once; the kernel leaves its head zero
-            ws = self._ws[stream] = torch.zeros(_lib.load().ee_paged_workspace_bytes(self._ref), dtype=torch.uint8,
-                                                device=self.device)
+        entry = self._ws.get(stream)
+        if entry is None:  # zeroed once; the kernel leaves its head zero
+            entry = self._ws[stream] = [torch.zeros(_lib.load().ee_paged_workspace_bytes(self._ref), dtype=torch.uint8,
+                                                    device=self.device), _lib.error_epoch]
+        elif entry[1] != _lib.error_epoch:  # a kernel that gave up may have left it otherwise
+            entry[0][:_lib.load().ee_paged_workspace_head_bytes()].zero_()
+            entry[1] = _lib.error_epoch
+        ws = entry[0]
         self._launch("ee_paged_attention", self._ref, step.ref, q.data_ptr(), ldq, heads,
                      self.head_dim ** -0.5 if scale is None else scale, y.data_ptr(), ldy, H.data_ptr(), ws.data_ptr(),
                      ws.numel())
