@@ -497,3 +497,27 @@ def test_workspace_after_an_error(pkg, cuda):
     got = c.attention(q, st)
     _ok(pkg)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("tier", [0, 2])
+@torch.no_grad()
+def test_rows_before_the_first_sequence(pkg, cuda, tier):
+    """cu[0] above zero: the rows before it belong to nobody and are neither read nor written."""
+    P, hk, hq, d, pad, e = 16, 2, 4, 64, 70, 45
+    g = torch.Generator(device=cuda).manual_seed(10)
+    k, v = _data(g, cuda, pad + e, hk, d)
+    c = _cache(pkg, cuda, [e], P, hk, d, tier)
+    st = pkg.PagedStep([0], [0], [pad + e], [e], cuda)
+    st.arrays[3] = pad  # seq, start, length, cu[0], cu[1]
+    c.reserve(0, e)
+    c._upload()
+    c.append(k, v, st)
+    q = torch.randn(pad + e, hq * d, generator=g, device=cuda).half()
+    out = torch.full((pad + e, hq * d), 7.0, dtype=torch.float16, device=cuda)
+    _, H = c.attention(q, st, out=out)
+    kk, vv = c.read(st)
+    _ok(pkg)
+    assert bool((out[:pad] == 7.0).all())
+    K, V = _held(k[pad:].view(e, hk, d), tier, P), _held(v[pad:].view(e, hk, d), tier, P)
+    assert torch.equal(kk[pad:], K.half().view(e, -1)) and torch.equal(vv[pad:], V.half().view(e, -1))
+    _check(out, H, pad, e, _attend64(q[pad:].view(e, hq, d), K, V, 0, d ** -0.5), hq, d)

@@ -37,22 +37,16 @@ namespace ee {
 __device__ int g_paged_error = 0;  // the paged kernels' error word (DeviceError bits)
 
 // ----------------------------------------------------------------------------------
-// order inside a page (elements from the start of the head's K or V part)
+// order inside a page
 // ----------------------------------------------------------------------------------
-template <int D, bool kWide>  // kWide: fp16 elements, else 8-bit
+// element of dimension d of token t from the start of a head's fp16 K part (16-byte units of 8
+// dimensions; the 8-bit K has units of 16)
+template <int D>
 __device__ __forceinline__ int page_k_offset(int t, int d) {
-  constexpr int E = kWide ? 8 : 16;  // elements per 16 bytes
   const int q4 = d / (D / 4), r = d % (D / 4);
-  const int piece = r / E;
+  const int piece = r / 8;
   const int lane = (t & 7) * 4 + q4;
-  return (t >> 4) * 16 * D + ((((t >> 3) & 1) * (D / 4 / E) + piece) * 32 + lane) * E + r % E;
-}
-template <int D, bool kWide>
-__device__ __forceinline__ int page_v_offset(int t, int d) {
-  const int gq = d / (D / 8), r = d % (D / 8), mb = r >> 1, j = r & 1;
-  const int th = (t >> 3) & 1, lane = gq * 4 + ((t & 7) >> 1), lo = t & 1;
-  if constexpr (kWide) return (t >> 4) * 16 * D + (mb * 32 + lane) * 8 + (th * 2 + j) * 2 + lo;
-  return (t >> 4) * 16 * D + ((mb >> 1) * 32 + lane) * 16 + (mb & 1) * 8 + th * 4 + j * 2 + lo;
+  return (t >> 4) * 16 * D + ((((t >> 3) & 1) * (D / 32) + piece) * 32 + lane) * 8 + r % 8;
 }
 
 __device__ __forceinline__ uint8_t* paged_block(const PagedArgs& c, int64_t page, int64_t h, int which) {
@@ -188,7 +182,11 @@ constexpr int kQTokens = 4;  // query rows per CTA
 // shared memory of an append CTA: the block's K and V rows, padded by 16 bytes
 __host__ __device__ constexpr size_t paged_stage_bytes(int page, int D) { return size_t(2) * page * (D + 8) * 2; }
 
-// One CTA per (touched block, KV head), then CTAs that rotate kQTokens rows of q.
+// One CTA per (touched block, KV head), then CTAs that rotate kQTokens rows of q.  The block's new
+// rows go through shared memory (a page's order takes 8 dimensions of a row apart), where an
+// open block that becomes complete joins them; the maxima are taken on the way in.  Bound by
+// loads in flight: 16774 tokens with 32 query / 8 KV heads of 128 (INT8, rotated) take 75 us,
+// 387 MB at 5.1 TB/s; one token 4.7 us, the chain of search, loads, stage and stores.
 template <int D, int TIER>
 __global__ void __launch_bounds__(kPagedAppendThreads, 4)
     paged_append_kernel(const PagedArgs c, const PagedStepArgs st, const PagedRows k, const PagedRows v,
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(kPagedAppendThreads, 4)
   }
   const int64_t blk0 = s.start >> c.page_shift, blk = blk0 + slot - paged_slot_base(st, b, c.page_shift);
   const int64_t end = s.start + s.n, p0 = blk << c.page_shift;
-  if (s.n == 0 || p0 >= end) return;
+  if (s.n == 0 || blk < blk0 || p0 >= end) return;  // (a slot that no block took)
   const int64_t blkN = (end - 1) >> c.page_shift;
   const int t0 = static_cast<int>(s.start > p0 ? s.start - p0 : 0);                // new tokens of the block: [t0, t1)
   const int t1 = static_cast<int>(end - p0 < P ? end - p0 : P);
@@ -291,7 +289,7 @@ __global__ void __launch_bounds__(kPagedAppendThreads, 4)
   auto store_wide = [&](__half* kd, __half* vd, int r0, int r1) {
     for (int i = tid; i < (r1 - r0) * VPR; i += kPagedAppendThreads) {
       const int t = r0 + i / VPR, d0 = (i % VPR) * 8;
-      *reinterpret_cast<uint4*>(kd + page_k_offset<D, true>(t, d0)) = *reinterpret_cast<const uint4*>(sk + t * LD + d0);
+      *reinterpret_cast<uint4*>(kd + page_k_offset<D>(t, d0)) = *reinterpret_cast<const uint4*>(sk + t * LD + d0);
     }
     const int g0 = r0 >> 4, g1 = (r1 + 15) >> 4;
     for (int i = tid; i < (g1 - g0) * 2 * D; i += kPagedAppendThreads) {  // 16-byte units of V
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(kPagedAppendThreads, 4)
       const __half* vo = paged_open(c, s.seq, blk, h, 1);
       for (int i = tid; i < t0 * VPR; i += kPagedAppendThreads) {
         const int t = i / VPR, d0 = (i % VPR) * 8;
-        const uint4 x = *reinterpret_cast<const uint4*>(ko + page_k_offset<D, true>(t, d0));
+        const uint4 x = *reinterpret_cast<const uint4*>(ko + page_k_offset<D>(t, d0));
         *reinterpret_cast<uint4*>(sk + t * LD + d0) = x;
         note(x, mk, bad_k);
       }
@@ -469,7 +467,7 @@ __device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& 
 }
 
 // One CTA per (touched block, KV head): the block's rows in the span, staged in shared memory
-// in token order, to k_out / v_out.
+// in token order, to k_out / v_out.  16774 tokens of 8 heads of 128 (INT8): 21 us, 103 MB.
 template <int D, int TIER>
 __global__ void __launch_bounds__(kPagedAppendThreads)
     paged_read_kernel(const PagedArgs c, const PagedStepArgs st, __half* __restrict__ k_out, int64_t ldk,
@@ -489,9 +487,9 @@ __global__ void __launch_bounds__(kPagedAppendThreads)
     if (tid == 0) atomicOr(&g_paged_error, kErrPage);
     return;
   }
-  const int64_t blk = (s.start >> c.page_shift) + slot - paged_slot_base(st, b, c.page_shift);
+  const int64_t blk0 = s.start >> c.page_shift, blk = blk0 + slot - paged_slot_base(st, b, c.page_shift);
   const int64_t end = s.start + s.n, p0 = blk << c.page_shift;
-  if (s.n == 0 || p0 >= end) return;
+  if (s.n == 0 || blk < blk0 || p0 >= end) return;  // (a slot that no block took)
   const int t0 = static_cast<int>(s.start > p0 ? s.start - p0 : 0);
   const int t1 = static_cast<int>(end - p0 < P ? end - p0 : P);
   __half* sk = reinterpret_cast<__half*>(paged_smem);
@@ -1022,7 +1020,10 @@ struct FewCfg {
 // of a part the warps' rows are joined, and a unit's last CTA joins its parts.
 // Bound by the cache's bytes: HBM's share of an SM is about 23 bytes a cycle, 11 cycles for the
 // K and V codes of a token (D 128); converting them (two ALU operations per fp16 pair) and the
-// MMAs take about 4.
+// MMAs take about 4.  6 sequences of 10 to 65 thousand tokens (FP8, 466 MB): 85.6 us, 5.4 TB/s;
+// 48 of 0.6 to 8 thousand (INT8, 431 MB): 86.5 us, 5.0 TB/s; one of 777: 13.7 us, latency.
+// Tickets, not a second launch, join a unit's parts; the first kernel of this form, with the
+// codes prefetched in registers instead of a ring, took 129, 127 and 26 us.
 // The open block's fp16 rows do not fit a stage of codes: the warps read them themselves.
 template <int D, int TIER, int NB, int RS>
 __global__ void __launch_bounds__(FewCfg<D, TIER, NB, RS>::kThreads, FewCfg<D, TIER, NB, RS>::kCtas)

@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         // its exponentials, in loops that stay rolled: unrolled over the tile, the code of the
         // roles on a scheduler runs out of its instruction cache (5 ragged chunks: 90.5 us
         // unrolled, 88.0 rolled; 2048 over 14000: 712 and 716; unrolled with two reads 831).
-        uint32_t r[32];
+        uint32_t r[32] = {};
         auto S = [&](int i) -> float { return __uint_as_float(r[i]); };
         auto load = [&](int k) {
           __syncwarp();
