@@ -468,7 +468,9 @@ int ee_device_check(int* value) {
     return fail(EE_ERR_CUDA, "reading the device error word failed");
   v |= paged;
   if (value) *value = v;
-  if (v != 0) return fail(EE_ERR_DEVICE, "device error word 0x%x (a bounded wait in a kernel gave up)", v);
+  if (v != 0)
+    return fail(EE_ERR_DEVICE, "device error word 0x%x (%s)", v,
+                v == ee::kErrPage ? "a paged step named what its cache does not have" : "a bounded wait in a kernel gave up");
   return EE_OK;
 }
 

@@ -9,11 +9,11 @@
 //
 // Blocks.  Tokens jP .. jP + P - 1 of a sequence are block j; table[seq][j] is its page.  In
 // an 8-bit tier a block is quantised when its last token arrives: s = max |x| / 127 (int8) or
-// / 448 (e4m3) over its P x D values of a head, code = rn(x / s) (IEEE
-// divisions: the codes are the same on every path that computes them).  Until then its tokens are in the sequence's
-// open buffer in fp16, slot j & 1; the block before it keeps its fp16 rows in the other slot.  So
-// the cache's contents depend on the tokens alone, not on how they were cut into appends, and
-// up to P tokens can be taken back exactly.  The fp16 tier writes tokens into their pages.
+// / 448 (e4m3) over its P x D values of a head, code = rn(x / s), both IEEE quotients.  Until
+// then its tokens are in the sequence's open buffer in fp16, slot j & 1; the block before it
+// keeps its fp16 rows in the other slot.  So the cache's contents depend on the tokens alone,
+// not on how they were cut into appends, and up to P tokens can be taken back exactly.  The
+// fp16 tier writes tokens into their pages.
 //
 // Order inside a page.  Tokens go in groups of 16, and a group's values lie in the order in
 // which a warp's lanes hold the operand of a 16 x 8 x 16 MMA: 16 bytes of lane 0, of lane 1, ..
